@@ -204,6 +204,133 @@ int tr_consume_silu_mul(float* g, float* u, void* out, int32_t out_dtype, int64_
 int tr_consume_add(const void* h, float* y, void* out, int32_t out_dtype, int64_t n,
                    void* stream);
 
+/* ---- Serving operators: what a decoder runs between the projections.  They take plain device
+ * pointers on the current device, launch on `stream`, allocate nothing, and refuse what they
+ * cannot do before any launch.  Strides are in elements; `dtype` values are tr_dtype.  They have
+ * no counterpart in the reference, whose chain leaves attention, norms and sampling out.       */
+
+/* The paged cache.  Keys and values live in two pools [pages][kv_heads][page_size][head_dim];
+ * request r's token at position p is in page tables[r][p / page_size], row p % page_size.  A
+ * slot is page * page_size + row.  Free page ids are a stack: free_pages[0 .. free_count).
+ *
+ * tr_plan_step gives pages to the tokens that every request brings in one step.  `lens[r]`
+ * tokens are cached, `new_tokens[r]` follow (negative values count as 0); the step's tokens are
+ * numbered request by request.
+ *   starts[requests + 1]  first token of each request (exclusive prefix sum of new_tokens)
+ *   granted[r]            1 when the request got its pages, else 0: a request is refused when
+ *                         its pages would pass `columns`, its tokens would pass `tokens`, or
+ *                         it needs pages and the need up to and including it is more than
+ *                         free_count
+ *   lens_out[r]           lens[r] + new_tokens[r], or lens[r] when refused
+ *   slots, positions      of the step's tokens [tokens]; -1 for tokens of refused requests
+ *                         and past the last token
+ *   tables                the new pages' entries are written; others stay
+ *   free_count_out[1]     free_count less the pages given; free_pages itself stays
+ * Pages are given in request order from the top of the stack down.  lens_out may be lens and
+ * free_count_out may be free_count (an update in place).  requests <= TR_STEP_MAX_REQUESTS. */
+#define TR_STEP_MAX_REQUESTS 16384
+int tr_plan_step(const int32_t* lens, const int32_t* new_tokens, int64_t requests,
+                 int32_t* tables, int64_t table_stride, int32_t columns,
+                 const int32_t* free_pages, int64_t pool, const int32_t* free_count,
+                 int32_t page_size, int64_t tokens, int64_t* slots, int32_t* positions,
+                 int32_t* starts, int32_t* lens_out, int32_t* granted, int32_t* free_count_out,
+                 void* stream);
+
+/* Returns the pages of the requests with finished[r] != 0 to the stack, in request and column
+ * order from its top up, and sets their table entries to -1 and their lens to 0.  free_pages
+ * has room for `pool` ids; what would pass it is dropped.  All in place.                       */
+int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t requests, int32_t* tables,
+                     int64_t table_stride, int32_t columns, int32_t* free_pages, int64_t pool,
+                     int32_t* free_count, int32_t page_size, void* stream);
+
+/* Writes keys and values k, v [tokens][kv_heads][head_dim] (token and head strides given, the
+ * last axis contiguous) to their slots in the pools.  src_dtype is the pools' dtype or TR_F32,
+ * rounded to it.  Tokens with a slot outside [0, pages * page_size) are skipped.  The slots of
+ * one call differ from each other.                                                           */
+int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                 int64_t v_token_stride, int64_t v_head_stride, int32_t src_dtype, void* k_pages,
+                 void* v_pages, int32_t dtype, const int64_t* slots, int64_t tokens,
+                 int32_t kv_heads, int32_t head_dim, int64_t pages, int32_t page_size,
+                 void* stream);
+
+/* Attention of each request's last tokens over its paged cache, causal:
+ *   out[t][h] = sum_j softmax_j(scale q[t][h] . K[j]) V[j],   j = 0 .. lens[r] - n_r + i
+ * for token t = starts[r] + i of request r, which brings n_r = starts[r + 1] - starts[r] tokens
+ * (already in the cache and counted in lens[r]).  Query head h reads kv head
+ * h / (heads / kv_heads).  A token that sees no key gets zeros and lse -inf.  lse [tokens][heads]
+ * (natural log of the sum of exponentials, fp32) may be NULL.  Tokens outside
+ * [starts[0], starts[requests]) get zeros and -inf as well.
+ * q: token and head strides given, the last axis contiguous, base and strides multiples of 16
+ * bytes; out [tokens][heads][head_dim] contiguous; tables, pools as above.  Table entries
+ * outside [0, pages) read as keys and values of zero; cache rows at and past lens[r] are not
+ * used whatever they hold.  head_dim is a multiple of 8 up to 256 (64 and 128 in fp16 and bf16
+ * run on tensor cores), page_size a power of two up to 1024, scale positive.
+ * The workspace holds the partial results of contexts that several thread blocks share; it is
+ * zeroed once (tr_workspace_clear) and left ready for the next call, and serves one stream at
+ * a time.                                                                                    */
+typedef struct tr_attention {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* starts;
+  void* out;
+  float* lse;
+  int64_t tokens, requests, pages;
+  int32_t columns, page_size, heads, kv_heads, head_dim, dtype;
+  float scale;
+} tr_attention;
+int tr_attention_workspace_bytes(const tr_attention* a, size_t* bytes);
+int tr_paged_attention(const tr_attention* a, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* The norms around a block's output y, with its gate and the scaled residual add:
+ *   h_out = residual_scale h + branch_scale gate * N_post(y)
+ *   x_out = N_pre(h_out)
+ * N(v) = v / sqrt(mean(v^2) + eps) * weight                       (TR_NORM_RMS)
+ *      = (v - mean v) / sqrt(var v + eps) * weight + bias         (TR_NORM_LAYER)
+ * per row of `width`.  y is NULL to norm h alone (h_out is then not written); post is NULL to
+ * add y as it is; pre is NULL to stop at h_out (x_out is then not written); gate is NULL for 1,
+ * else one row (gate_stride 0) or one per token; biases may be NULL.  y is in dtype or fp32
+ * (y_dtype); h, gate, weights, biases and outputs are in dtype; rows are contiguous along the
+ * width with the given row strides; h_out and x_out are contiguous.  The sums are fp32 and x_out
+ * is normed from the unrounded h_out.  h_out may be h when h's rows are contiguous.            */
+enum tr_norm_kind { TR_NORM_RMS = 0, TR_NORM_LAYER = 1 };
+typedef struct tr_norm {
+  const void* y;
+  const void* h;
+  const void* gate;
+  const void* post;
+  const void* post_bias;
+  const void* pre;
+  const void* pre_bias;
+  void* h_out;
+  void* x_out;
+  int64_t tokens, width, y_stride, h_stride, gate_stride;
+  int32_t kind, dtype, y_dtype;
+  float eps, residual_scale, branch_scale;
+} tr_norm;
+int tr_residual_norm(const tr_norm* n, void* stream);
+
+/* The next token of every row of logits [rows][vocab] from given random numbers.
+ * t = logits / temperature (logits where temperature <= 0), and of the softmax of t are kept
+ *   the top_k greatest (0 or less: all), ties to the lower index;
+ *   of these the shortest run in falling order whose mass reaches top_p of theirs (>= 1: all);
+ *   of these the ones of at least min_p times the greatest probability;
+ * the greatest always stays unless it is -inf.  The token is the kept one with the greatest
+ * t - log(noise), noise [rows][vocab] ~ Exp(1), which draws it with its probability among the
+ * kept; where temperature <= 0 the one with the greatest t; ties go to the lower index.  NaN
+ * logits count as -inf.  tokens[row] is -1 when every logit is -inf.  logprobs[row] (may be
+ * NULL) is the log of the token's probability in the softmax of t over the whole row, -inf with
+ * token -1.  top_k, top_p and min_p may be NULL (no such limit).                             */
+int tr_sample(const void* logits, int32_t dtype, int64_t logits_stride, const float* noise,
+              int64_t noise_stride, const float* temperature, const int32_t* top_k,
+              const float* top_p, const float* min_p, int64_t rows, int64_t vocab,
+              int64_t* tokens, float* logprobs, void* stream);
+
 /* The geometry tr_forward would use for `tokens` (after clamping to this device). */
 int tr_plan_tiling(const tr_plan* plan, int64_t tokens, tr_tiling* out);
 

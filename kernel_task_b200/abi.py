@@ -4,7 +4,7 @@ integers (``tensor.data_ptr()``), streams are ``cudaStream_t`` handles as intege
 from __future__ import annotations
 
 import ctypes
-from ctypes import (POINTER, c_char_p, c_double, c_int, c_int32, c_int64, c_size_t,
+from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t,
                     c_uint32, c_void_p)
 
 from ._native import LIBRARY
@@ -19,6 +19,8 @@ TR_ERR_TIMEOUT = -6
 TR_F32, TR_F16, TR_BF16 = 0, 1, 2
 KERNEL_AUTO, KERNEL_GENERIC, KERNEL_MMA, KERNEL_TC05, KERNEL_DECODE, KERNEL_SLAB = 0, 1, 2, 3, 4, 5
 TR_EPI_NONE, TR_EPI_ADD, TR_EPI_SILU_MUL = 0, 1, 2
+TR_NORM_RMS, TR_NORM_LAYER = 0, 1
+TR_STEP_MAX_REQUESTS = 16384
 
 
 class TrSpec(ctypes.Structure):
@@ -33,6 +35,25 @@ class TrTiling(ctypes.Structure):
 class TrEpilogue(ctypes.Structure):
     _fields_ = [("kind", c_int32), ("out_dtype", c_int32), ("aux", c_void_p),
                 ("aux_dtype", c_int32)]
+
+
+class TrAttention(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+                ("k_pages", c_void_p), ("v_pages", c_void_p), ("tables", c_void_p),
+                ("table_stride", c_int64), ("lens", c_void_p), ("starts", c_void_p),
+                ("out", c_void_p), ("lse", c_void_p), ("tokens", c_int64), ("requests", c_int64),
+                ("pages", c_int64), ("columns", c_int32), ("page_size", c_int32),
+                ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("dtype", c_int32), ("scale", c_float)]
+
+
+class TrNorm(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("y", "h", "gate", "post", "post_bias", "pre", "pre_bias",
+                                        "h_out", "x_out")] + \
+               [(n, c_int64) for n in ("tokens", "width", "y_stride", "h_stride",
+                                       "gate_stride")] + \
+               [("kind", c_int32), ("dtype", c_int32), ("y_dtype", c_int32), ("eps", c_float),
+                ("residual_scale", c_float), ("branch_scale", c_float)]
 
 
 # name -> (restype, argtypes); every function declared in include/trring.h
@@ -59,6 +80,19 @@ PROTOTYPES = {
                                     c_void_p]),
     "tr_consume_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_void_p]),
     "tr_consume_add": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_void_p]),
+    "tr_plan_step": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                             c_int64, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tr_release_pages": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                 c_void_p, c_int64, c_void_p, c_int32, c_void_p]),
+    "tr_append_kv": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                             c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int32,
+                             c_int64, c_int32, c_void_p]),
+    "tr_attention_workspace_bytes": (c_int, [POINTER(TrAttention), POINTER(c_size_t)]),
+    "tr_paged_attention": (c_int, [POINTER(TrAttention), c_void_p, c_size_t, c_void_p]),
+    "tr_residual_norm": (c_int, [POINTER(TrNorm), c_void_p]),
+    "tr_sample": (c_int, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                          c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "tr_plan_tiling": (c_int, [c_void_p, c_int64, POINTER(TrTiling)]),
     "tr_plan_describe": (c_int, [c_void_p, c_char_p, c_size_t]),
     "tr_plan_flops_per_token": (c_int, [c_void_p, POINTER(c_double)]),

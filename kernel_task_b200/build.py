@@ -20,7 +20,10 @@ LIB = PKG / "libtrring.so"
 EXT = PKG / "_trring_torch.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CUDA_SOURCES = ["plan.cpp", "pack.cu", "ring_generic.cu", "ring_mma.cu", "ring_decode.cu",
-                "ring_tc05.cu", "ring_slab.cu", "consume.cu"]
+                "ring_tc05.cu", "ring_slab.cu", "consume.cu", "serve_step.cu", "serve_attend.cu",
+                "serve_norm.cu", "serve_sample.cu"]
+
+BINDING_SOURCES = ["torch_ext.cpp", "torch_serve.cpp"]
 
 
 def _nvcc() -> str:
@@ -31,7 +34,7 @@ def _nvcc() -> str:
 
 def build_library(verbose: bool = False) -> Path:
     """nvcc -> libtrring.so (all kernels + the C ABI)."""
-    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+    cmd = [_nvcc(), *ARCH, "--threads=0", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
            f"-I{INCLUDE}", "-o", str(LIB), *[str(CSRC / s) for s in CUDA_SOURCES]]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
@@ -48,7 +51,7 @@ def build_torch_binding(verbose: bool = False) -> Path:
     build_dir.mkdir(exist_ok=True)
     cpp_extension.load(
         name="_trring_torch",
-        sources=[str(CSRC / "torch_ext.cpp")],
+        sources=[str(CSRC / s) for s in BINDING_SOURCES],
         extra_include_paths=[str(INCLUDE)],
         extra_cflags=["-O3"],
         # ninja turns $$ into $ and the shell turns \$ into $: the rpath reads $ORIGIN:$ORIGIN/..

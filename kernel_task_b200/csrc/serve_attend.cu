@@ -1,0 +1,166 @@
+// tr_paged_attention: attention of each request's last tokens over its paged cache.
+#include <algorithm>
+#include <cmath>
+
+#include "serve_util.cuh"
+
+namespace trr {
+
+// The request of token t: the last one that starts at or before it, or -1 outside all of them.
+__device__ __forceinline__ int owner_of(const int32_t* starts, int requests, int64_t t) {
+  if (requests == 0 || t < starts[0] || t >= starts[requests]) return -1;
+  int lo = 0, hi = requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Any head_dim and type: one warp per token and query head, lane l holding elements
+// l, l + 32, ... of q and of the running output, one pass over the keys with the running maximum
+// and sum.  Bound by the five-step reduction of every key's product.
+template <typename E, int N>
+__global__ void __launch_bounds__(128) attend_generic_kernel(const tr_attention a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  if (w >= a.tokens * a.heads) return;
+  const int64_t t = w / a.heads;
+  const int h = (int)(w - t * a.heads), kvh = h / (a.heads / a.kv_heads);
+  const int r = owner_of(a.starts, (int)a.requests, t);
+  int64_t keys = 0;
+  if (r >= 0) {
+    const int64_t len = min((int64_t)a.lens[r], (int64_t)a.columns * a.page_size);
+    keys = min(len, (int64_t)a.lens[r] - (a.starts[r + 1] - a.starts[r]) + (t - a.starts[r]) + 1);
+  }
+  const E* q = static_cast<const E*>(a.q) + t * a.q_token_stride + h * a.q_head_stride;
+  float qf[N], o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = i * 32 + lane;
+    qf[i] = d < a.head_dim ? to_f32<E>(q[d]) * a.scale : 0.f;
+    o[i] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  for (int64_t j = 0; j < keys; ++j) {
+    const int id = a.tables[r * a.table_stride + j / a.page_size];
+    const bool held = id >= 0 && id < a.pages;
+    const int64_t at =
+        (((int64_t)id * a.kv_heads + kvh) * a.page_size + j % a.page_size) * a.head_dim;
+    const E* k = static_cast<const E*>(a.k_pages) + at;
+    const E* v = static_cast<const E*>(a.v_pages) + at;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = i * 32 + lane;
+      if (held && d < a.head_dim) s = fmaf(qf[i], to_f32<E>(k[d]), s);
+    }
+    s = warp_sum(s);
+    const float top = fmaxf(m, s), keep = __expf(m - top), p = __expf(s - top);
+    m = top;
+    l = l * keep + p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = i * 32 + lane;
+      o[i] = o[i] * keep + (held && d < a.head_dim ? p * to_f32<E>(v[d]) : 0.f);
+    }
+  }
+  const float inv = keys > 0 ? 1.f / l : 0.f;
+  E* out = static_cast<E*>(a.out) + (t * a.heads + h) * a.head_dim;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = i * 32 + lane;
+    if (d < a.head_dim) out[d] = from_f32<E>(o[i] * inv);
+  }
+  if (a.lse && lane == 0) a.lse[t * a.heads + h] = keys > 0 ? m + logf(l) : -INFINITY;
+}
+
+template <typename E>
+static int launch_generic_attention(const tr_attention& a, void* stream) {
+  const int64_t blocks = (a.tokens * a.heads + 3) / 4;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.head_dim <= 64) attend_generic_kernel<E, 2><<<(unsigned)blocks, 128, 0, s>>>(a);
+  else if (a.head_dim <= 128) attend_generic_kernel<E, 4><<<(unsigned)blocks, 128, 0, s>>>(a);
+  else attend_generic_kernel<E, 8><<<(unsigned)blocks, 128, 0, s>>>(a);
+  return serve_launched("tr_paged_attention");
+}
+
+static int check_attention(const tr_attention* a) {
+  if (!a) {
+    set_error("tr_paged_attention: null argument");
+    return TR_ERR_INVALID;
+  }
+  if (!known_dtype(a->dtype)) {
+    set_error("tr_paged_attention: unknown dtype %d", (int)a->dtype);
+    return TR_ERR_INVALID;
+  }
+  if (a->tokens < 0 || a->requests < 0 || a->pages < 0 || a->columns < 0 || a->kv_heads < 1 ||
+      a->heads < 1 || a->heads % a->kv_heads) {
+    set_error("tr_paged_attention: bad shape (%d query heads over %d)", (int)a->heads,
+              (int)a->kv_heads);
+    return TR_ERR_INVALID;
+  }
+  if (a->requests > 1 && a->table_stride < a->columns) {
+    set_error("tr_paged_attention: table stride %lld below its %d columns",
+              (long long)a->table_stride, (int)a->columns);
+    return TR_ERR_INVALID;
+  }
+  if (!(a->scale > 0.f) || std::isinf(a->scale)) {
+    set_error("tr_paged_attention: scale must be positive and finite");
+    return TR_ERR_INVALID;
+  }
+  if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) {
+    set_error("tr_paged_attention: head_dim %d (a multiple of 8 up to 256)", (int)a->head_dim);
+    return TR_ERR_UNSUPPORTED;
+  }
+  if (a->page_size < 1 || a->page_size > 1024 || (a->page_size & (a->page_size - 1))) {
+    set_error("tr_paged_attention: page_size %d (a power of two up to 1024)", (int)a->page_size);
+    return TR_ERR_UNSUPPORTED;
+  }
+  if ((int64_t)a->columns * a->page_size > (int64_t)1 << 30 ||
+      a->tokens * a->heads > (int64_t)1 << 31 || a->requests > (int64_t)1 << 20 ||
+      a->pages > INT32_MAX) {
+    set_error("tr_paged_attention: too large (a request's cache up to 2^30 tokens, tokens x heads "
+              "up to 2^31, 2^20 requests)");
+    return TR_ERR_UNSUPPORTED;
+  }
+  if (a->tokens == 0) return TR_OK;
+  if (!a->q || !a->out ||
+      (a->requests > 0 && (!a->lens || !a->starts || (a->columns > 0 && !a->tables))) ||
+      (a->pages > 0 && (!a->k_pages || !a->v_pages))) {
+    set_error("tr_paged_attention: null pointer");
+    return TR_ERR_INVALID;
+  }
+  const int eb = element_bytes(a->dtype);
+  if ((((uintptr_t)a->q | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->out) & 15) ||
+      ((a->q_token_stride * eb | a->q_head_stride * eb) & 15)) {
+    set_error("tr_paged_attention: q (base and strides), pools and out must be 16-byte aligned");
+    return TR_ERR_ALIGN;
+  }
+  return TR_OK;
+}
+
+}  // namespace trr
+
+using namespace trr;
+
+extern "C" int tr_attention_workspace_bytes(const tr_attention* a, size_t* bytes) {
+  const int st = check_attention(a);
+  if (st != TR_OK) return st;
+  if (!bytes) {
+    set_error("tr_attention_workspace_bytes: null pointer");
+    return TR_ERR_INVALID;
+  }
+  *bytes = 0;
+  return TR_OK;
+}
+
+extern "C" int tr_paged_attention(const tr_attention* a, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const int st = check_attention(a);
+  if (st != TR_OK || a->tokens == 0) return st;
+  if (a->dtype == TR_F32) return launch_generic_attention<float>(*a, stream);
+  if (a->dtype == TR_F16) return launch_generic_attention<__half>(*a, stream);
+  return launch_generic_attention<__nv_bfloat16>(*a, stream);
+}

@@ -1,0 +1,373 @@
+// The paged cache's bookkeeping and writes: block tables and slot maps of a step
+// (tr_plan_step), pages given back (tr_release_pages), keys and values written to their slots
+// (tr_append_kv).
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "serve_util.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace trr {
+
+struct StepArgs {
+  const int32_t* lens;
+  const int32_t* brings;
+  int32_t* tables;
+  int64_t table_stride;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* starts;
+  int32_t* lens_out;
+  int32_t* granted;
+  int32_t* free_count_out;
+  int64_t pool, tokens;
+  int requests, columns, page;
+};
+
+constexpr int kStepThreads = 1024;
+
+__device__ __forceinline__ int64_t pages_of(int64_t n, int page) { return (n + page - 1) / page; }
+
+// Every block of the one cluster runs the same two prefix sums over the requests (tokens, then
+// pages needed), which costs less than a second launch or a barrier to share them, and then
+// takes its share of the tables' new entries and of the step's tokens.  A token finds its request by
+// bisection of the starts in shared memory; its page is read from the table when the request
+// held it before, else from the free stack, so no block waits for the entries another writes.
+// What the caller may ask for in place (lens, free_count) is written after the cluster barrier
+// that follows the last read.  Bound by latency: launch, two scans, one dependent table load.
+__global__ void __launch_bounds__(kStepThreads, 1) plan_step_kernel(const StepArgs a) {
+  extern __shared__ int32_t step_smem[];
+  int32_t* start = step_smem;                  // [requests + 1]
+  int32_t* base = step_smem + a.requests + 1;  // pages given before this request's; -1 refused
+  __shared__ int64_t part[32];
+  __shared__ int used;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+  const int tid = threadIdx.x;
+  if (tid == 0) used = 0;
+  const int64_t fc = min(max((int64_t)*a.free_count, (int64_t)0), a.pool);
+  int64_t tokens_before = 0, need_before = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += kStepThreads) {
+    const int r = r0 + tid;
+    const bool live = r < a.requests;
+    const int64_t len = live ? max(a.lens[r], 0) : 0, n = live ? max(a.brings[r], 0) : 0;
+    int64_t total;
+    const int64_t through = block_scan_inclusive(n, part, total) + tokens_before;
+    tokens_before += total;
+    const int64_t held = pages_of(len, a.page), wants = pages_of(len + n, a.page);
+    const bool fits = live && wants <= a.columns && through <= a.tokens;
+    const int64_t need = fits ? wants - held : 0;
+    const int64_t taken = block_scan_inclusive(need, part, total) + need_before;
+    need_before += total;
+    const bool ok = fits && (need == 0 || taken <= fc);
+    if (live) {
+      start[r] = (int32_t)min(through - n, (int64_t)INT32_MAX);
+      base[r] = ok ? (int32_t)(taken - need) : -1;
+      if (ok && need > 0) atomicMax(&used, (int)taken);
+    }
+  }
+  if (tid == 0) start[a.requests] = (int32_t)min(tokens_before, (int64_t)INT32_MAX);
+  __syncthreads();
+
+  // new table entries, a warp per request
+  const int warps = kStepThreads / 32, lane = tid & 31;
+  for (int r = rank * warps + (tid >> 5); r < a.requests; r += ranks * warps) {
+    const int b = base[r];
+    if (b < 0) continue;
+    const int64_t len = max(a.lens[r], 0), n = start[r + 1] - start[r];
+    const int held = (int)pages_of(len, a.page), wants = (int)pages_of(len + n, a.page);
+    for (int c = held + lane; c < wants; c += 32)
+      a.tables[r * a.table_stride + c] = a.free_pages[fc - 1 - (b + c - held)];
+  }
+  for (int64_t i = (int64_t)rank * kStepThreads + tid; i < a.tokens;
+       i += (int64_t)ranks * kStepThreads) {
+    int64_t slot = -1;
+    int position = -1;
+    if (i < start[a.requests]) {
+      int lo = 0, hi = a.requests;  // the last request that starts at or before i
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      if (base[lo] >= 0) {
+        const int64_t len = max(a.lens[lo], 0);
+        const int64_t p = len + i - start[lo];
+        const int64_t c = p / a.page, held = pages_of(len, a.page);
+        const int64_t id = c < held ? a.tables[lo * a.table_stride + c]
+                                    : a.free_pages[fc - 1 - (base[lo] + c - held)];
+        slot = id * a.page + (p - c * a.page);
+        position = (int)p;
+      }
+    }
+    a.slots[i] = slot;
+    a.positions[i] = position;
+  }
+  cluster.sync();
+  if (rank == 0) {
+    for (int r = tid; r <= a.requests; r += kStepThreads) {
+      a.starts[r] = start[r];
+      if (r == a.requests) break;
+      a.granted[r] = base[r] >= 0;
+      const int len = a.lens[r];
+      a.lens_out[r] = base[r] >= 0 ? max(len, 0) + start[r + 1] - start[r] : len;
+    }
+    if (tid == 0) *a.free_count_out = (int32_t)(fc - used);
+  }
+}
+
+struct ReleaseArgs {
+  int32_t* lens;
+  const int32_t* finished;
+  int32_t* tables;
+  int64_t table_stride;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int64_t pool;
+  int requests, columns, page;
+};
+
+// As plan_step_kernel: the prefix sum of the pages given back in every block, then a warp per
+// request moves them.
+__global__ void __launch_bounds__(kStepThreads, 1) release_pages_kernel(const ReleaseArgs a) {
+  extern __shared__ int32_t step_smem[];  // [requests] pages given back before this request's
+  __shared__ int64_t part[32];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+  const int tid = threadIdx.x;
+  const int64_t fc = min(max((int64_t)*a.free_count, (int64_t)0), a.pool);
+  const auto held = [&](int r) {
+    return a.finished[r] ? min(pages_of(max(a.lens[r], 0), a.page), (int64_t)a.columns)
+                         : (int64_t)0;
+  };
+  int64_t before = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += kStepThreads) {
+    const int r = r0 + tid;
+    const int64_t n = r < a.requests ? held(r) : 0;
+    int64_t total;
+    const int64_t through = block_scan_inclusive(n, part, total) + before;
+    before += total;
+    if (r < a.requests) step_smem[r] = (int32_t)min(through - n, a.pool);
+  }
+  __syncthreads();
+  const int warps = kStepThreads / 32, lane = tid & 31;
+  for (int r = rank * warps + (tid >> 5); r < a.requests; r += ranks * warps) {
+    const int n = (int)held(r);
+    for (int c = lane; c < n; c += 32) {
+      const int64_t at = fc + step_smem[r] + c;
+      int32_t* entry = a.tables + r * a.table_stride + c;
+      if (at < a.pool) a.free_pages[at] = *entry;
+      *entry = -1;
+    }
+  }
+  cluster.sync();
+  if (rank == 0) {
+    for (int r = tid; r < a.requests; r += kStepThreads)
+      if (a.finished[r]) a.lens[r] = 0;
+    if (tid == 0) *a.free_count = (int32_t)min(fc + before, a.pool);
+  }
+}
+
+// One launch of a single cluster of `blocks`.
+template <typename Args>
+static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, size_t smem,
+                          void* stream, const char* what) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+      set_error("%s: %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(e));
+      return TR_ERR_CUDA;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kStepThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  if (e != cudaSuccess) {
+    set_error("%s launch: %s", what, cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return TR_ERR_CUDA;
+  }
+  return TR_OK;
+}
+
+// ---- tr_append_kv
+struct AppendArgs {
+  const void* src[2];
+  void* dst[2];
+  int64_t token_stride[2], head_stride[2];
+  const int64_t* slots;
+  int64_t tokens, slots_end;
+  int heads, dim, page;
+};
+
+// One thread per 8 elements (V = 8, 16-byte stores) or per element (V = 1, when a source row is
+// not 16-byte aligned).  blockIdx.y: keys or values.  Bound by memory at large sizes (a source
+// element read, a pool element written), by the launch at small ones.
+template <typename S, typename E, int V>
+__global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs a) {
+  const int which = blockIdx.y;
+  const S* src = static_cast<const S*>(a.src[which]);
+  E* dst = static_cast<E*>(a.dst[which]);
+  const int per_head = a.dim / V, per_token = a.heads * per_head;
+  const int64_t n = a.tokens * per_token;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / per_token;
+    const int rest = (int)(i - t * per_token), h = rest / per_head, d = (rest - h * per_head) * V;
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.slots_end) continue;
+    const int64_t page = slot / a.page;
+    const S* from = src + t * a.token_stride[which] + h * a.head_stride[which] + d;
+    E* to = dst + ((page * a.heads + h) * a.page + (slot - page * a.page)) * a.dim + d;
+    if constexpr (V == 8) {
+      float f[8];
+      load8<S>(from, f);
+      store8<E>(to, f);
+    } else {
+      *to = from_f32<E>(to_f32<S>(*from));
+    }
+  }
+}
+
+template <typename S, typename E>
+static int launch_append(const AppendArgs& a, bool wide, void* stream) {
+  const int64_t n = a.tokens * a.heads * (a.dim / (wide ? 8 : 1));
+  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)serve_sms() * 16), 2);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide) append_kv_kernel<S, E, 8><<<grid, 256, 0, s>>>(a);
+  else append_kv_kernel<S, E, 1><<<grid, 256, 0, s>>>(a);
+  return serve_launched("tr_append_kv");
+}
+
+}  // namespace trr
+
+using namespace trr;
+
+static int check_step(const char* what, int64_t requests, const void* a, const void* b,
+                      const void* tables, int64_t table_stride, int32_t columns,
+                      const void* free_pages, int64_t pool, const void* free_count,
+                      int32_t page_size) {
+  if (requests < 0 || columns < 0 || pool < 0 || page_size < 1) {
+    set_error("%s: negative size, or page_size %d below 1", what, (int)page_size);
+    return TR_ERR_INVALID;
+  }
+  if (requests > 1 && table_stride < columns) {
+    set_error("%s: table stride %lld below its %d columns", what, (long long)table_stride,
+              (int)columns);
+    return TR_ERR_INVALID;
+  }
+  if (pool > INT32_MAX) {
+    set_error("%s: pool of %lld pages (at most 2^31 - 1)", what, (long long)pool);
+    return TR_ERR_INVALID;
+  }
+  if (requests > TR_STEP_MAX_REQUESTS) {
+    set_error("%s: %lld requests (at most %d)", what, (long long)requests, TR_STEP_MAX_REQUESTS);
+    return TR_ERR_UNSUPPORTED;
+  }
+  if ((requests > 0 && (!a || !b || (columns > 0 && !tables))) || (pool > 0 && !free_pages) ||
+      !free_count) {
+    set_error("%s: null pointer", what);
+    return TR_ERR_INVALID;
+  }
+  return TR_OK;
+}
+
+extern "C" int tr_plan_step(const int32_t* lens, const int32_t* new_tokens, int64_t requests,
+                            int32_t* tables, int64_t table_stride, int32_t columns,
+                            const int32_t* free_pages, int64_t pool, const int32_t* free_count,
+                            int32_t page_size, int64_t tokens, int64_t* slots, int32_t* positions,
+                            int32_t* starts, int32_t* lens_out, int32_t* granted,
+                            int32_t* free_count_out, void* stream) {
+  const int st = check_step("tr_plan_step", requests, lens, new_tokens, tables, table_stride,
+                            columns, free_pages, pool, free_count, page_size);
+  if (st != TR_OK) return st;
+  if (tokens < 0 || tokens > INT32_MAX) {
+    set_error("tr_plan_step: %lld tokens (0 to 2^31 - 1)", (long long)tokens);
+    return TR_ERR_INVALID;
+  }
+  if (!starts || !free_count_out || (requests > 0 && (!lens_out || !granted)) ||
+      (tokens > 0 && (!slots || !positions))) {
+    set_error("tr_plan_step: null output");
+    return TR_ERR_INVALID;
+  }
+  StepArgs a = {lens, new_tokens, tables, table_stride, free_pages, free_count, slots, positions,
+                starts, lens_out, granted, free_count_out, pool, tokens, (int)requests, columns,
+                page_size};
+  // one block serves a decode step; the cluster of 8 pays its barrier back from a few tokens
+  // per thread on
+  const int blocks = tokens + requests > 4 * kStepThreads ? 8 : 1;
+  return launch_cluster(plan_step_kernel, a, blocks, (2 * requests + 1) * sizeof(int32_t), stream,
+                        "tr_plan_step");
+}
+
+extern "C" int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t requests,
+                                int32_t* tables, int64_t table_stride, int32_t columns,
+                                int32_t* free_pages, int64_t pool, int32_t* free_count,
+                                int32_t page_size, void* stream) {
+  const int st = check_step("tr_release_pages", requests, lens, finished, tables, table_stride,
+                            columns, free_pages, pool, free_count, page_size);
+  if (st != TR_OK || requests == 0) return st;
+  ReleaseArgs a = {lens, finished, tables, table_stride, free_pages, free_count, pool,
+                   (int)requests, columns, page_size};
+  const int blocks = requests * columns > 4 * kStepThreads ? 8 : 1;
+  return launch_cluster(release_pages_kernel, a, blocks, requests * sizeof(int32_t), stream,
+                        "tr_release_pages");
+}
+
+extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                            const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                            int32_t src_dtype, void* k_pages, void* v_pages, int32_t dtype,
+                            const int64_t* slots, int64_t tokens, int32_t kv_heads,
+                            int32_t head_dim, int64_t pages, int32_t page_size, void* stream) {
+  if (!known_dtype(dtype) || (src_dtype != dtype && src_dtype != TR_F32)) {
+    set_error("tr_append_kv: source dtype %d into dtype %d", (int)src_dtype, (int)dtype);
+    return TR_ERR_INVALID;
+  }
+  if (tokens < 0 || kv_heads < 1 || head_dim < 1 || pages < 0 || page_size < 1 ||
+      (int64_t)kv_heads * head_dim > INT32_MAX) {
+    set_error("tr_append_kv: bad shape");
+    return TR_ERR_INVALID;
+  }
+  if (tokens == 0 || pages == 0) return TR_OK;
+  if (!k || !v || !k_pages || !v_pages || !slots) {
+    set_error("tr_append_kv: null pointer");
+    return TR_ERR_INVALID;
+  }
+  const int sb = element_bytes(src_dtype), db = element_bytes(dtype);
+  if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) {
+    set_error("tr_append_kv: the pools must be 16-byte aligned");
+    return TR_ERR_ALIGN;
+  }
+  if ((((uintptr_t)k | (uintptr_t)v) & (sb - 1)) || ((uintptr_t)slots & 7)) {
+    set_error("tr_append_kv: a pointer is not aligned to its elements");
+    return TR_ERR_ALIGN;
+  }
+  AppendArgs a = {{k, v}, {k_pages, v_pages}, {k_token_stride, v_token_stride},
+                  {k_head_stride, v_head_stride}, slots, tokens, pages * page_size, kv_heads,
+                  head_dim, page_size};
+  const bool wide = head_dim % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) &&
+                    !((k_token_stride * sb | k_head_stride * sb | v_token_stride * sb |
+                       v_head_stride * sb) & 15);
+  if (src_dtype == TR_F32) {
+    if (dtype == TR_F32) return launch_append<float, float>(a, wide, stream);
+    if (dtype == TR_F16) return launch_append<float, __half>(a, wide, stream);
+    return launch_append<float, __nv_bfloat16>(a, wide, stream);
+  }
+  if (dtype == TR_F16) return launch_append<__half, __half>(a, wide, stream);
+  (void)db;
+  return launch_append<__nv_bfloat16, __nv_bfloat16>(a, wide, stream);
+}

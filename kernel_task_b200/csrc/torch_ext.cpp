@@ -15,26 +15,15 @@
 #include <string>
 #include <vector>
 
+#include "torch_ext.h"
 #include "trring.h"
 
 namespace py = pybind11;
 
 namespace {
 
-[[noreturn]] void raise_status(int st, const char* what) {
-  std::string msg = std::string(what) + ": " + tr_status_string(st) + " (" + tr_last_error() + ")";
-  if (st == TR_ERR_INVALID) throw py::value_error(msg);
-  throw std::runtime_error(msg);
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return TR_F32;
-    case at::kHalf: return TR_F16;
-    case at::kBFloat16: return TR_BF16;
-    default: return -1;
-  }
-}
+using trr_torch::dtype_code;
+using trr_torch::raise_status;
 
 class RingOp {
  public:
@@ -387,4 +376,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dtype") = at::kBFloat16, "silu(g) * u (fp32 inputs, cleared) -> dtype");
   m.def("consume_add", &consume_add, py::arg("h"), py::arg("y"),
         "h + y (y fp32, cleared) -> h's dtype");
+  trr_torch::bind_serving(m);
 }
