@@ -2,21 +2,9 @@
 #include <algorithm>
 #include <cmath>
 
-#include "serve_util.cuh"
+#include "serve_attend.cuh"
 
 namespace trr {
-
-// The request of token t: the last one that starts at or before it, or -1 outside all of them.
-__device__ __forceinline__ int owner_of(const int32_t* starts, int requests, int64_t t) {
-  if (requests == 0 || t < starts[0] || t >= starts[requests]) return -1;
-  int lo = 0, hi = requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 // Any head_dim and type: one warp per token and query head, lane l holding elements
 // l, l + 32, ... of q and of the running output, one pass over the keys with the running maximum
@@ -86,6 +74,14 @@ static int launch_generic_attention(const tr_attention& a, void* stream) {
   return serve_launched("tr_paged_attention");
 }
 
+static size_t workspace_need(const tr_attention& a) {
+  return attend_partials_bytes() + attend_rows_counters(a) * sizeof(int);
+}
+
+static bool on_tensor_cores(const tr_attention& a) {
+  return a.dtype != TR_F32 && (a.head_dim == 64 || a.head_dim == 128);
+}
+
 static int check_attention(const tr_attention* a) {
   if (!a) {
     set_error("tr_paged_attention: null argument");
@@ -152,7 +148,7 @@ extern "C" int tr_attention_workspace_bytes(const tr_attention* a, size_t* bytes
     set_error("tr_attention_workspace_bytes: null pointer");
     return TR_ERR_INVALID;
   }
-  *bytes = 0;
+  *bytes = a->tokens > 0 && on_tensor_cores(*a) ? workspace_need(*a) : 0;
   return TR_OK;
 }
 
@@ -160,6 +156,18 @@ extern "C" int tr_paged_attention(const tr_attention* a, void* workspace, size_t
                                   void* stream) {
   const int st = check_attention(a);
   if (st != TR_OK || a->tokens == 0) return st;
+  if (on_tensor_cores(*a)) {
+    const size_t need = workspace_need(*a);
+    if (!workspace || workspace_bytes < need) {
+      set_error("tr_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+      return TR_ERR_WORKSPACE;
+    }
+    if ((uintptr_t)workspace & 15) {
+      set_error("tr_paged_attention: the workspace must be 16-byte aligned");
+      return TR_ERR_ALIGN;
+    }
+    return launch_attend_rows(*a, workspace, stream);
+  }
   if (a->dtype == TR_F32) return launch_generic_attention<float>(*a, stream);
   if (a->dtype == TR_F16) return launch_generic_attention<__half>(*a, stream);
   return launch_generic_attention<__nv_bfloat16>(*a, stream);

@@ -1,0 +1,79 @@
+// Shared by the paged-attention kernels (serve_attend.cu, serve_attend_rows.cu,
+// serve_attend_chunk.cu).
+#pragma once
+
+#include "serve_util.cuh"
+
+namespace trr {
+
+// The request of token t: the last one that starts at or before it, or -1 outside all of them.
+__device__ __forceinline__ int owner_of(const int32_t* starts, int requests, int64_t t) {
+  if (requests == 0 || t < starts[0] || t >= starts[requests]) return -1;
+  int lo = 0, hi = requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Tokens a request brings and keys it has, kept inside the arrays whatever starts and lens hold.
+__device__ __forceinline__ int brought(const tr_attention& a, int r) {
+  const int64_t first = max((int64_t)a.starts[r], (int64_t)0);
+  return (int)min(max((int64_t)a.starts[r + 1] - first, (int64_t)0), max(a.tokens - first, (int64_t)0));
+}
+__device__ __forceinline__ int cached(const tr_attention& a, int r) {
+  return (int)min((int64_t)max(a.lens[r], 0), (int64_t)a.columns * a.page_size);
+}
+// Keys that token i of request r's n sees: lens[r] - n + i + 1, at most those cached.
+__device__ __forceinline__ int visible(const tr_attention& a, int r, int n, int i) {
+  return (int)min((int64_t)a.lens[r] - n + i + 1, (int64_t)cached(a, r));
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 bytes global -> shared, asynchronously; zeros when !held (src is then not read)
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool held) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
+               "r"(held ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Zeros and -inf for the tokens outside [starts[0], starts[requests]); `thread` of `threads`.
+template <typename E>
+__device__ void clear_outside(const tr_attention& a, int64_t thread, int64_t threads) {
+  const int64_t first = a.requests ? min(max((int64_t)a.starts[0], (int64_t)0), a.tokens) : a.tokens;
+  const int64_t end = a.requests ? min(max((int64_t)a.starts[a.requests], first), a.tokens) : a.tokens;
+  const int64_t outside = first + (a.tokens - end);
+  const int64_t per = (int64_t)a.heads * a.head_dim / 8;
+  for (int64_t i = thread; i < outside * per; i += threads) {
+    const int64_t n = i / per, t = n < first ? n : end + (n - first);
+    reinterpret_cast<uint4*>(a.out)[t * per + (i - n * per)] = make_uint4(0, 0, 0, 0);
+  }
+  if (a.lse)
+    for (int64_t i = thread; i < outside * a.heads; i += threads) {
+      const int64_t n = i / a.heads, t = n < first ? n : end + (n - first);
+      a.lse[t * a.heads + (i - n * a.heads)] = -INFINITY;
+    }
+}
+
+// The workspace: partial results, of one size for every call on a device, then the items' arrival
+// counters, which are zero between calls whatever the shapes of the calls were.
+// serve_attend_rows.cu
+size_t attend_partials_bytes();
+size_t attend_rows_counters(const tr_attention& a);
+int launch_attend_rows(const tr_attention& a, void* workspace, void* stream);
+
+}  // namespace trr
