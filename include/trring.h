@@ -265,9 +265,13 @@ int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, c
  * outside [0, pages) read as keys and values of zero; cache rows at and past lens[r] are not
  * used whatever they hold.  head_dim is a multiple of 8 up to 256 (64 and 128 in fp16 and bf16
  * run on tensor cores), page_size a power of two up to 1024, scale positive.
- * The workspace holds the partial results of contexts that several thread blocks share; it is
- * zeroed once (tr_workspace_clear) and left ready for the next call, and serves one stream at
- * a time.                                                                                    */
+ * The workspace holds the partial results of contexts that several thread blocks share; its
+ * first TR_ATTENTION_STATE_BYTES are zeroed once (tr_workspace_clear) and left ready for the
+ * next call, of whatever shape; it serves one stream at a time.  Waits inside the kernels are
+ * bounded (wait_polls polls, 0 = built-in limit of about a second): one that runs out ends the
+ * kernel with TR_ERR_TIMEOUT in the status word (tr_workspace_status); out is then not valid,
+ * and the state is zeroed again before the next call.                                        */
+#define TR_ATTENTION_STATE_BYTES ((1 << 20) + 256)
 typedef struct tr_attention {
   const void* q;
   int64_t q_token_stride, q_head_stride;
@@ -282,6 +286,7 @@ typedef struct tr_attention {
   int64_t tokens, requests, pages;
   int32_t columns, page_size, heads, kv_heads, head_dim, dtype;
   float scale;
+  uint32_t wait_polls;
 } tr_attention;
 int tr_attention_workspace_bytes(const tr_attention* a, size_t* bytes);
 int tr_paged_attention(const tr_attention* a, void* workspace, size_t workspace_bytes,

@@ -21,6 +21,7 @@ KERNEL_AUTO, KERNEL_GENERIC, KERNEL_MMA, KERNEL_TC05, KERNEL_DECODE, KERNEL_SLAB
 TR_EPI_NONE, TR_EPI_ADD, TR_EPI_SILU_MUL = 0, 1, 2
 TR_NORM_RMS, TR_NORM_LAYER = 0, 1
 TR_STEP_MAX_REQUESTS = 16384
+TR_ATTENTION_STATE_BYTES = (1 << 20) + 256
 
 
 class TrSpec(ctypes.Structure):
@@ -44,7 +45,7 @@ class TrAttention(ctypes.Structure):
                 ("out", c_void_p), ("lse", c_void_p), ("tokens", c_int64), ("requests", c_int64),
                 ("pages", c_int64), ("columns", c_int32), ("page_size", c_int32),
                 ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
-                ("dtype", c_int32), ("scale", c_float)]
+                ("dtype", c_int32), ("scale", c_float), ("wait_polls", c_uint32)]
 
 
 class TrNorm(ctypes.Structure):

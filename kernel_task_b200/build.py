@@ -21,7 +21,7 @@ EXT = PKG / "_trring_torch.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CUDA_SOURCES = ["plan.cpp", "pack.cu", "ring_generic.cu", "ring_mma.cu", "ring_decode.cu",
                 "ring_tc05.cu", "ring_slab.cu", "consume.cu", "serve_step.cu", "serve_attend.cu",
-                "serve_attend_rows.cu", "serve_norm.cu", "serve_sample.cu"]
+                "serve_attend_rows.cu", "serve_attend_chunk.cu", "serve_norm.cu", "serve_sample.cu"]
 
 BINDING_SOURCES = ["torch_ext.cpp", "torch_serve.cpp"]
 

@@ -74,12 +74,14 @@ static int launch_generic_attention(const tr_attention& a, void* stream) {
   return serve_launched("tr_paged_attention");
 }
 
-static size_t workspace_need(const tr_attention& a) {
-  return attend_partials_bytes() + attend_rows_counters(a) * sizeof(int);
-}
-
 static bool on_tensor_cores(const tr_attention& a) {
   return a.dtype != TR_F32 && (a.head_dim == 64 || a.head_dim == 128);
+}
+
+// The chunk kernel from 32 query rows a request and kv head on average, of which its tiles hold
+// 256; the rows kernel below that, where reading the keys is the bound.
+static bool in_chunks(const tr_attention& a) {
+  return a.tokens * (a.heads / a.kv_heads) > 32 * a.requests;
 }
 
 static int check_attention(const tr_attention* a) {
@@ -116,9 +118,10 @@ static int check_attention(const tr_attention* a) {
   }
   if ((int64_t)a->columns * a->page_size > (int64_t)1 << 30 ||
       a->tokens * a->heads > (int64_t)1 << 31 || a->requests > (int64_t)1 << 20 ||
-      a->pages > INT32_MAX) {
+      a->pages > INT32_MAX ||
+      (double)a->pages * a->kv_heads * a->page_size >= 4294967295.) {
     set_error("tr_paged_attention: too large (a request's cache up to 2^30 tokens, tokens x heads "
-              "up to 2^31, 2^20 requests)");
+              "up to 2^31, 2^20 requests, pools below 2^32 rows)");
     return TR_ERR_UNSUPPORTED;
   }
   if (a->tokens == 0) return TR_OK;
@@ -137,6 +140,16 @@ static int check_attention(const tr_attention* a) {
   return TR_OK;
 }
 
+static int workspace_need(const tr_attention& a, size_t* bytes) {
+  const bool chunks = in_chunks(a);
+  if ((chunks ? attend_chunk_items(a) : attend_rows_items(a)) > kAttendCounters) {
+    set_error("tr_paged_attention: over %lld tiles of query rows", (long long)kAttendCounters);
+    return TR_ERR_UNSUPPORTED;
+  }
+  *bytes = TR_ATTENTION_STATE_BYTES + (chunks ? attend_chunk_partials(a) : attend_rows_partials(a));
+  return TR_OK;
+}
+
 }  // namespace trr
 
 using namespace trr;
@@ -148,8 +161,8 @@ extern "C" int tr_attention_workspace_bytes(const tr_attention* a, size_t* bytes
     set_error("tr_attention_workspace_bytes: null pointer");
     return TR_ERR_INVALID;
   }
-  *bytes = a->tokens > 0 && on_tensor_cores(*a) ? workspace_need(*a) : 0;
-  return TR_OK;
+  *bytes = 0;
+  return a->tokens > 0 && on_tensor_cores(*a) ? workspace_need(*a, bytes) : TR_OK;
 }
 
 extern "C" int tr_paged_attention(const tr_attention* a, void* workspace, size_t workspace_bytes,
@@ -157,7 +170,9 @@ extern "C" int tr_paged_attention(const tr_attention* a, void* workspace, size_t
   const int st = check_attention(a);
   if (st != TR_OK || a->tokens == 0) return st;
   if (on_tensor_cores(*a)) {
-    const size_t need = workspace_need(*a);
+    size_t need = 0;
+    const int short_of = workspace_need(*a, &need);
+    if (short_of != TR_OK) return short_of;
     if (!workspace || workspace_bytes < need) {
       set_error("tr_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
       return TR_ERR_WORKSPACE;
@@ -166,7 +181,10 @@ extern "C" int tr_paged_attention(const tr_attention* a, void* workspace, size_t
       set_error("tr_paged_attention: the workspace must be 16-byte aligned");
       return TR_ERR_ALIGN;
     }
-    return launch_attend_rows(*a, workspace, stream);
+    char* w = static_cast<char*>(workspace);
+    const AttendWorkspace ws = {reinterpret_cast<int*>(w), reinterpret_cast<int*>(w + 256),
+                                reinterpret_cast<float*>(w + TR_ATTENTION_STATE_BYTES)};
+    return in_chunks(*a) ? launch_attend_chunk(*a, ws, stream) : launch_attend_rows(*a, ws, stream);
   }
   if (a->dtype == TR_F32) return launch_generic_attention<float>(*a, stream);
   if (a->dtype == TR_F16) return launch_generic_attention<__half>(*a, stream);

@@ -69,11 +69,22 @@ __device__ void clear_outside(const tr_attention& a, int64_t thread, int64_t thr
     }
 }
 
-// The workspace: partial results, of one size for every call on a device, then the items' arrival
-// counters, which are zero between calls whatever the shapes of the calls were.
-// serve_attend_rows.cu
-size_t attend_partials_bytes();
-size_t attend_rows_counters(const tr_attention& a);
-int launch_attend_rows(const tr_attention& a, void* workspace, void* stream);
+// The workspace: the status word (tr_workspace_status), the arrival counters of the items, which
+// are zero between calls, and the partial results, which need not be.  The first two have a size
+// of their own, so that calls of any shapes can follow one another.
+constexpr int64_t kAttendCounters = (TR_ATTENTION_STATE_BYTES - 256) / sizeof(int);
+struct AttendWorkspace {
+  int* status;
+  int* counters;
+  float* partials;
+};
+
+// serve_attend_rows.cu, serve_attend_chunk.cu: counters and bytes of partial results of a call
+int64_t attend_rows_items(const tr_attention& a);
+size_t attend_rows_partials(const tr_attention& a);
+int launch_attend_rows(const tr_attention& a, const AttendWorkspace& ws, void* stream);
+int64_t attend_chunk_items(const tr_attention& a);
+size_t attend_chunk_partials(const tr_attention& a);
+int launch_attend_chunk(const tr_attention& a, const AttendWorkspace& ws, void* stream);
 
 }  // namespace trr

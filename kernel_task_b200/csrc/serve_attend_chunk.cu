@@ -1,0 +1,645 @@
+// Paged attention for many query rows per request and kv head: prompts and chunks of them, on
+// the 5th-generation tensor cores.
+//
+// A row is one token and query head; the rows of a request over one kv head, token-major, are
+// cut into tiles of 256, so all the heads that share keys share their loads.  A tile is two
+// subtiles of 128 rows, each with its own scores S and output O in tensor memory:
+//     S = Q K^T   (128 x 128 keys, K-major operands in shared memory, 128-byte swizzle)
+//     O += P V    (P from tensor memory, where it takes the place of S; V is read with its
+//                  head_dim contiguous, the MN-major form of the same layout)
+// Warps 0-3 and 4-7 each hold a subtile's softmax, a thread per row: running maximum and sum in
+// registers, P rounded to the values' type.  O is rescaled only when a row's maximum grew by
+// more than 2^8 since the last time; P is then at most 256 and the fp32 sums keep their bits.
+// Warp 8 issues the products, alternating the subtiles so that one's softmax runs under the
+// other's products; warps 9 and 10 bring keys and values, 128 rows at a time, through a ring of
+// shared-memory slots with cp.async (zeros past the keys: a page's unused rows may hold
+// anything, and 0 * NaN would reach O).
+//
+// Split.  An item is (request, row tile, kv head), a unit one block of 128 keys that the tile
+// sees; kItemUnits more stand in front of them for what an item costs besides (queries, the
+// first scores, the outputs: as long as about 3 blocks).  The grid is one block per SM (all of tensor memory), and each takes an equal contiguous
+// run of all units, as in serve_attend_rows.cu; partial results of shared items are joined by
+// the last block to arrive, in unit order.
+//
+// Every wait is bounded: when one runs out the block raises its abort flag, all roles leave
+// their loops, tensor memory is freed and the workspace's status word says TR_ERR_TIMEOUT.
+#include <algorithm>
+
+#include "serve_attend.cuh"
+#include "tc_util.cuh"
+
+namespace trr {
+
+constexpr int kBlockKeys = 128;
+constexpr int kSubRows = 128, kTileRows = 2 * kSubRows;
+constexpr int kChunkThreads = 11 * 32;
+constexpr int kMinChunkUnits = 6;  // units a grid block takes at least
+constexpr int kItemUnits = 3;
+constexpr unsigned kChunkWaitPolls = 1u << 21;
+
+template <int D>
+__host__ __device__ constexpr int ring_slots() {
+  return D == 128 ? 5 : 8;
+}
+template <int D>
+__host__ __device__ constexpr int loads_in_flight() {
+  return D == 128 ? 2 : 4;
+}
+template <int D>
+__host__ __device__ constexpr int slot_bytes() {
+  return kBlockKeys * D * 2;
+}
+template <int D>
+__host__ __device__ constexpr int chunk_smem() {
+  return 1024 + 2 * kSubRows * D * 2 + ring_slots<D>() * slot_bytes<D>();
+}
+
+template <>
+__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+}
+
+// tcgen05.mma with A in tensor memory, issued by one elected lane of a converged warp
+__device__ __forceinline__ void umma_ts_one(uint32_t dtmem, uint32_t atmem, uint64_t db,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(
+          dtmem),
+      "r"(atmem), "l"(db), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+// Keys and values of a slot: [head_dim / 64][128 rows][128 bytes], 16-byte chunks swizzled by
+// row & 7.  Values as the MN-major operand: 64-element column groups 16 KB apart, groups of 8
+// keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_values(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(kBlockKeys * 128 >> 4) << 16 |
+         (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// Walks the items of a contiguous run of units.
+struct ChunkItem {
+  int request, n, rows, tiles, tile, kvh, units;  // units: kItemUnits, then the blocks of keys
+  int64_t u0;     // first unit of the item
+  int64_t index;  // item number
+};
+__device__ __forceinline__ int tile_units(const tr_attention& a, int r, int n, int g, int tile,
+                                          int rows) {
+  const int last = min((tile + 1) * kTileRows, rows) - 1;
+  return max((visible(a, r, n, last / g) + kBlockKeys - 1) / kBlockKeys, 1) + kItemUnits;
+}
+__device__ __forceinline__ void open_request(const tr_attention& a, int g, ChunkItem& it, int r) {
+  it.request = r;
+  it.n = brought(a, r);
+  it.rows = it.n * g;
+  it.tiles = (it.rows + kTileRows - 1) / kTileRows;
+  it.tile = it.kvh = 0;
+  it.units = it.tiles ? tile_units(a, r, it.n, g, 0, it.rows) : 0;
+}
+__device__ __forceinline__ void next_item(const tr_attention& a, int g, ChunkItem& it) {
+  it.u0 += it.units;
+  ++it.index;
+  if (++it.kvh < a.kv_heads) return;
+  it.kvh = 0;
+  if (++it.tile < it.tiles) {
+    it.units = tile_units(a, it.request, it.n, g, it.tile, it.rows);
+    return;
+  }
+  while (it.request + 1 < (int)a.requests) {
+    open_request(a, g, it, it.request + 1);
+    if (it.tiles) return;
+  }
+}
+// The blocks of keys of `it` inside [u, u_end), and u past them.
+struct Segment {
+  int first, last;  // last: one past
+};
+__device__ __forceinline__ Segment take(const ChunkItem& it, int64_t& u, int64_t u_end) {
+  const int lo = (int)(u - it.u0), hi = (int)min((int64_t)it.units, u_end - it.u0);
+  u = it.u0 + hi;
+  return {max(lo - kItemUnits, 0), max(hi - kItemUnits, 0)};
+}
+
+enum {
+  B_FULL = 0,        // [8] a slot's rows have arrived
+  B_EMPTY = 8,       // [8] the products have read a slot
+  B_QUERY = 16,      // [2] a subtile's queries are in shared memory
+  B_SCORES = 18,     // [2] S is in tensor memory
+  B_PROBS = 20,      // [2] P has taken its place, O is rescaled
+  B_OUT = 22,        // [2] O is complete
+  B_LEFT = 24,       // [2] a subtile's partial result is written
+  B_JOIN = 26,       // [2] whether this block joins the item is known
+  B_DRAIN = 28,
+  B_COUNT = 29
+};
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    attend_chunk_kernel(const tr_attention a, int* status, int* counters, int64_t max_items,
+                        float* partials, unsigned wait_polls) {
+  constexpr int NS = ring_slots<D>(), FLIGHT = loads_in_flight<D>();
+  constexpr int QBYTES = kSubRows * D * 2, SLOT = slot_bytes<D>(), CPR = D / 8;
+  constexpr int64_t PARTIAL = (int64_t)kTileRows * (D + 2);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int64_t scan_part[32], scan_items[32];
+  __shared__ uint64_t bars[B_COUNT];
+  __shared__ ChunkItem first_item;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int sh_abort, sh_join[2];
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = a.heads / a.kv_heads, R = (int)a.requests;
+  clear_outside<E>(a, (int64_t)blockIdx.x * kChunkThreads + tid, (int64_t)gridDim.x * kChunkThreads);
+  if (R == 0) return;
+
+  // ---- this block's run of units
+  const int per = (R + kChunkThreads - 1) / kChunkThreads;
+  const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
+  int64_t my_units = 0, my_items = 0;
+  for (int r = r_lo; r < r_hi; ++r) {
+    ChunkItem it;
+    open_request(a, g, it, r);
+    my_items += (int64_t)it.tiles * a.kv_heads;
+    for (int t = 0; t < it.tiles; ++t)
+      my_units += (int64_t)tile_units(a, r, it.n, g, t, it.rows) * a.kv_heads;
+  }
+  int64_t U, all_items;
+  const int64_t through = block_scan_inclusive(my_units, scan_part, U);
+  const int64_t items_through = block_scan_inclusive(my_items, scan_items, all_items);
+  if (U == 0 || all_items > max_items) return;
+  const int64_t G = min((int64_t)gridDim.x, (U + kMinChunkUnits - 1) / kMinChunkUnits);
+  if (blockIdx.x >= G) return;
+  const int64_t u_begin = U * blockIdx.x / G, u_end = U * (blockIdx.x + 1) / G;
+  if (through - my_units <= u_begin && u_begin < through) {
+    ChunkItem it;
+    it.u0 = through - my_units;
+    it.index = items_through - my_items;
+    for (int r = r_lo; r < r_hi; ++r) {
+      open_request(a, g, it, r);
+      int64_t units = 0;
+      for (; it.tile < it.tiles; ++it.tile) {
+        it.units = tile_units(a, r, it.n, g, it.tile, it.rows);
+        units = (int64_t)it.units * a.kv_heads;
+        if (u_begin < it.u0 + units) break;
+        it.u0 += units;
+        it.index += a.kv_heads;
+      }
+      if (it.tile < it.tiles) break;
+    }
+    it.kvh = (int)((u_begin - it.u0) / it.units);
+    it.u0 += (int64_t)it.kvh * it.units;
+    it.index += it.kvh;
+    first_item = it;
+  }
+
+  // ---- set-up
+  const auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (warp == 9) {
+    if (lane < B_COUNT) {
+      int count = 1;
+      if (lane < B_EMPTY) count = 2;  // the two loading warps
+      if (lane == B_QUERY || lane == B_QUERY + 1 || lane == B_PROBS || lane == B_PROBS + 1 ||
+          lane == B_LEFT || lane == B_LEFT + 1)
+        count = 4;  // the subtile's four warps
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar(lane)), "r"(count)
+                   : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_async_smem();
+    if (lane == 0) sh_abort = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t qbase = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t ring = qbase + 2 * QBYTES;
+  volatile int* abort = &sh_abort;
+  const auto wait = [&](int b, uint32_t parity) {
+    return warp_wait(bar(b), parity, abort, wait_polls);
+  };
+  ChunkItem it = first_item;
+  const int page_shift = 31 - __clz(a.page_size);
+
+  if (warp < 8) {
+    // ---- softmax: subtile t, row `row` of it
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + t * 128 + lanes, o_tmem = tmem + 256 + t * D + lanes;
+    const float scale2 = a.scale * kLog2e;
+    uint32_t uses = 0, scores = 0, lefts = 0;  // completed phases of this subtile's barriers
+    for (int64_t u = u_begin; u < u_end; next_item(a, g, it)) {
+      const Segment seg = take(it, u, u_end);
+      const int b_first = seg.first, b_last = seg.last;
+      if (b_first == b_last) continue;  // only the units in front
+      const int row0 = it.tile * kTileRows + t * kSubRows;
+      const int rows_here = min(it.rows - row0, kSubRows);
+      if (rows_here <= 0) continue;  // the item has one subtile
+      const bool live = row < rows_here;
+      const int i = (row0 + row) / g, h = it.kvh * g + (row0 + row - i * g);
+      const int64_t token = (int64_t)max(a.starts[it.request], 0) + i;
+      const int limit = live ? visible(a, it.request, it.n, i) : 0;
+      const bool warp_live = (warp & 3) * 32 < rows_here;
+
+      // queries, zeros past the rows
+      {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) +
+                                                        token * a.q_token_stride +
+                                                        h * a.q_head_stride);
+        uint8_t* dst = smem_raw + (qbase - smem_u32(smem_raw)) + t * QBYTES + row * 128;
+#pragma unroll
+        for (int c = 0; c < CPR; ++c)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kSubRows * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+              live ? q[c] : make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_QUERY + t));
+      }
+
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int b = b_first; b < b_last; ++b) {
+        if (!(ok = wait(B_SCORES + t, scores & 1))) break;
+        ++scores;
+        tc_fence_after();
+        if (warp_live) {
+          uint32_t s[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            tmem_ld<32>(s_tmem + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+          tmem_wait_ld();
+          const int seen = limit - b * kBlockKeys;
+          if (__any_sync(0xffffffffu, seen < kBlockKeys)) {
+#pragma unroll
+            for (int k = 0; k < 128; ++k) s[k] = k < seen ? s[k] : __float_as_uint(-INFINITY);
+          }
+          float top = __uint_as_float(s[0]);
+#pragma unroll
+          for (int k = 1; k < 128; ++k) top = fmaxf(top, __uint_as_float(s[k]));
+          top *= scale2;
+          // a new base where the old one would let P pass 2^8
+          const bool rise = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
+          if (__any_sync(0xffffffffu, rise)) {
+            const float keep = !rise ? 1.f : m == -INFINITY ? 0.f : exp2_approx(m - top);
+            if (rise) m = top;
+            l *= keep;
+            if (b > b_first) {
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld<16>(o_tmem + c * 16, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                tmem_st16(o_tmem + c * 16, o);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float p0 = exp2_approx(fmaf(__uint_as_float(s[c * 32 + 2 * k]), scale2, -base));
+              const float p1 = exp2_approx(fmaf(__uint_as_float(s[c * 32 + 2 * k + 1]), scale2, -base));
+              sum += p0 + p1;
+              p[k] = pack2<E>(p0, p1);
+            }
+            tmem_st16(s_tmem + c * 16, p);
+          }
+          l += sum;
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PROBS + t));
+      }
+      if (!ok || !wait(B_OUT + t, uses & 1)) break;
+      tc_fence_after();
+
+      const bool shared_item = b_last - b_first < it.units - kItemUnits;
+      // the grid blocks with the item's first and last block of keys
+      const int64_t first_block = ((it.u0 + kItemUnits + 1) * G - 1) / U;
+      const int64_t last_block = ((it.u0 + it.units) * G - 1) / U;
+      const auto slot = [&](int64_t c) {
+        return partials + (2 * c + (U * c / G < it.u0 ? 1 : 0)) * PARTIAL;
+      };
+      bool writes = true;
+      if (shared_item) {
+        // partial result: [D / 4][256 rows] float4, then maxima and sums
+        float* mine = slot(blockIdx.x);
+        const int at = t * kSubRows + row;
+        if (warp_live) {
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld<16>(o_tmem + c * 16, o);
+            tmem_wait_ld();
+            if (live) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                __stcg(reinterpret_cast<float4*>(mine) + (c * 4 + k) * kTileRows + at,
+                       make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                   __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3])));
+            }
+          }
+          if (live) {
+            __stcg(mine + (int64_t)kTileRows * D + at, m);
+            __stcg(mine + (int64_t)kTileRows * (D + 1) + at, l);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          __threadfence();
+          mbar_arrive(bar(B_LEFT + t));
+        }
+        __syncwarp();
+        if ((warp & 3) == 0) {
+          ok = wait(B_LEFT + t, lefts & 1);
+          if (lane == 0) {
+            int* counter = counters + it.index * 2 + t;
+            const int last = ok ? atom_add_acq_rel_gpu(counter, 1) : -1;
+            sh_join[t] = last == (int)(last_block - first_block);
+            if (sh_join[t]) *counter = 0;
+            mbar_arrive(bar(B_JOIN + t));
+          }
+          __syncwarp();
+        }
+        if (!wait(B_JOIN + t, lefts & 1)) break;
+        ++lefts;
+        writes = sh_join[t];
+        __threadfence();
+        if (writes && warp_live) {
+          if (live) {
+            // half the columns at a time: 16 loads of a part in flight
+            const float* maxima = partials + (int64_t)kTileRows * D + at;
+            const float* sums = maxima + kTileRows;
+            const auto part = [&](int64_t c) { return slot(c) - partials; };
+            float top = -INFINITY;
+#pragma unroll 4
+            for (int64_t c = first_block; c <= last_block; ++c)
+              top = fmaxf(top, __ldcg(maxima + part(c)));
+            const float base = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
+#pragma unroll 4
+            for (int64_t c = first_block; c <= last_block; ++c)
+              sum += exp2_approx(__ldcg(maxima + part(c)) - base) * __ldcg(sums + part(c));
+            m = top;
+            l = sum;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            E* out = static_cast<E*>(a.out) + (token * a.heads + h) * D;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 64) {
+              float acc[64];
+#pragma unroll
+              for (int k = 0; k < 64; ++k) acc[k] = 0.f;
+#pragma unroll 1
+              for (int64_t c = first_block; c <= last_block; ++c) {
+                const float f = exp2_approx(__ldcg(maxima + part(c)) - base);
+                float4 v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  v[k] = __ldcg(reinterpret_cast<const float4*>(slot(c)) +
+                                (c0 / 4 + k) * kTileRows + at);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  acc[4 * k] += f * v[k].x, acc[4 * k + 1] += f * v[k].y;
+                  acc[4 * k + 2] += f * v[k].z, acc[4 * k + 3] += f * v[k].w;
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = acc[8 * k + j] * inv;
+                store8<E>(out + c0 + k * 8, v);
+              }
+            }
+          }
+        }
+      } else if (warp_live) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        E* out = static_cast<E*>(a.out) + (token * a.heads + h) * D;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld<16>(o_tmem + c * 16, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[8 * k + j]) * inv;
+              store8<E>(out + c * 16 + k * 8, v);
+            }
+          }
+        }
+      }
+      if (writes && live && a.lse)
+        a.lse[token * a.heads + h] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      ++uses;
+      tc_fence_before();  // O and Q are free for the next item once B_QUERY and B_PROBS arrive
+    }
+  } else if (warp == 8) {
+    // ---- products
+    constexpr uint32_t idesc_s = umma_idesc<E>(kSubRows, kBlockKeys);
+    constexpr uint32_t idesc_o = umma_idesc<E>(kSubRows, D) | 1u << 16;  // values: MN-major
+    uint32_t x = 0;                     // slots taken so far
+    uint32_t items_done[2] = {0, 0}, probs[2] = {0, 0};
+    const auto scores = [&](int t, uint32_t slot) {
+      const uint32_t q = qbase + t * QBYTES, k = ring + slot * SLOT;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t in = (ks & 3) * 32;
+        umma_one(tmem + t * 128, desc_sw128(q + (ks >> 2) * (kSubRows * 128) + in),
+                 desc_sw128(k + (ks >> 2) * (kBlockKeys * 128) + in), idesc_s, ks > 0);
+      }
+      commit_one(bar(B_SCORES + t));
+    };
+    bool ok = true;
+    for (int64_t u = u_begin; ok && u < u_end; next_item(a, g, it)) {
+      const Segment seg = take(it, u, u_end);
+      const int b_first = seg.first, b_last = seg.last;
+      if (b_first == b_last) continue;  // only the units in front
+      const int subs = it.rows - it.tile * kTileRows > kSubRows ? 2 : 1;
+      uint32_t slot_k = x % NS;
+      ok = wait(B_FULL + slot_k, (x / NS) & 1);
+      for (int t = 0; ok && t < subs; ++t) {
+        if (!(ok = wait(B_QUERY + t, items_done[t] & 1))) break;
+        ++items_done[t];
+        tc_fence_after();
+        scores(t, slot_k);
+      }
+      if (!ok) break;
+      commit_one(bar(B_EMPTY + slot_k));
+      ++x;
+      for (int b = b_first; ok && b < b_last; ++b) {
+        const uint32_t slot_v = x % NS, next_k = (x + 1) % NS;
+        const bool more = b + 1 < b_last;
+        if (!(ok = wait(B_FULL + slot_v, (x / NS) & 1))) break;
+        for (int t = 0; t < subs; ++t) {
+          if (!(ok = wait(B_PROBS + t, probs[t] & 1))) break;
+          ++probs[t];
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kBlockKeys / 16; ++ks)
+            umma_ts_one(tmem + 256 + t * D, tmem + t * 128 + ks * 8,
+                        desc_values(ring + slot_v * SLOT + ks * 2048), idesc_o,
+                        b > b_first || ks > 0);
+          if (more) {
+            if (t == 0 && !(ok = wait(B_FULL + next_k, ((x + 1) / NS) & 1))) break;
+            scores(t, next_k);
+          } else {
+            commit_one(bar(B_OUT + t));
+          }
+        }
+        if (!ok) break;
+        commit_one(bar(B_EMPTY + slot_v));
+        if (more) commit_one(bar(B_EMPTY + next_k));
+        x += more ? 2 : 1;
+      }
+    }
+    // whatever was issued has to end before tensor memory is freed
+    commit_one(bar(B_DRAIN));
+    mbar_drain_spin(bar(B_DRAIN), 0);
+  } else {
+    // ---- loads: warp w brings rows 64 w .. 64 w + 63 of every block of keys and of values
+    const int w = warp - 9;
+    uint32_t x = 0;
+    bool ok = true;
+    const uint4* pools[2] = {static_cast<const uint4*>(a.k_pages),
+                             static_cast<const uint4*>(a.v_pages)};
+    // a lane's destination inside a slot: chunk c of row 64 w + lane / CPR, and the rows below it
+    const int c = lane % CPR, sub = lane / CPR;
+    constexpr int RPI = 32 / CPR;  // rows an instruction of the warp covers
+    for (int64_t u = u_begin; ok && u < u_end; next_item(a, g, it)) {
+      const Segment seg = take(it, u, u_end);
+      const int b_first = seg.first, b_last = seg.last;
+      if (b_first == b_last) continue;  // only the units in front
+      const int rows_tile = min(it.rows - it.tile * kTileRows, kTileRows);
+      const int keys_end =
+          max(visible(a, it.request, it.n, (it.tile * kTileRows + rows_tile - 1) / g), 0);
+      const int32_t* table = a.tables + it.request * a.table_stride;
+      // pool rows of keys 64 w + lane and + 32 of block b; ~0u past the keys and for bad pages
+      uint32_t rows[2], next[2];
+      const auto find = [&](int b, uint32_t (&r)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = b * kBlockKeys + w * 64 + j * 32 + lane;
+          const int id = b < b_last && key < keys_end ? table[key >> page_shift] : -1;
+          r[j] = id >= 0 && id < a.pages
+                     ? (uint32_t)((id * a.kv_heads + it.kvh) * (int64_t)a.page_size +
+                                  (key & (a.page_size - 1)))
+                     : ~0u;
+        }
+      };
+      find(b_first, rows);
+      for (int b = b_first; ok && b < b_last; ++b) {
+        find(b + 1, next);
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          if (x >= FLIGHT) {  // the oldest load in flight has arrived: hand it over
+            copies_wait<FLIGHT - 1>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_FULL + (x - FLIGHT) % NS));
+          }
+          const uint32_t slot = x % NS;
+          if (x >= NS && !(ok = wait(B_EMPTY + slot, (x / NS - 1) & 1))) break;
+          const uint32_t dst = ring + slot * SLOT + w * 64 * 128 + (c >> 3) * (kBlockKeys * 128);
+          const uint4* pool = pools[which];
+#pragma unroll
+          for (int i = 0; i < 64 / RPI; ++i) {
+            const int rr = i * RPI + sub;
+            const uint32_t r = __shfl_sync(0xffffffffu, rows[i * RPI / 32], rr & 31);
+            const bool held = r != ~0u;
+            copy16_async(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4),
+                         pool + (uint64_t)(held ? r : 0u) * CPR + c, held);
+          }
+          copies_commit();
+          ++x;
+        }
+        rows[0] = next[0];
+        rows[1] = next[1];
+      }
+    }
+    copies_wait<0>();
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0 && ok)
+      for (uint32_t i = x > FLIGHT ? x - FLIGHT : 0; i < x; ++i) mbar_arrive(bar(B_FULL + i % NS));
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+  if (tid == 0 && sh_abort) atomicExch(status, (int)TR_ERR_TIMEOUT);
+}
+
+// ---- host
+int64_t attend_chunk_items(const tr_attention& a) {
+  return 2 * (a.tokens * (a.heads / a.kv_heads) / kTileRows + a.requests) * a.kv_heads;
+}
+size_t attend_chunk_partials(const tr_attention& a) {
+  return (size_t)serve_sms() * 2 * kTileRows * (a.head_dim + 2) * sizeof(float);
+}
+
+template <typename E, int D>
+static int launch_chunk(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
+  auto kernel = attend_chunk_kernel<E, D>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem<D>());
+  if (e != cudaSuccess) {
+    set_error("tr_paged_attention: %d bytes of shared memory: %s", chunk_smem<D>(),
+              cudaGetErrorString(e));
+    return TR_ERR_CUDA;
+  }
+  kernel<<<serve_sms(), kChunkThreads, chunk_smem<D>(), static_cast<cudaStream_t>(stream)>>>(
+      a, ws.status, ws.counters, attend_chunk_items(a) / 2, ws.partials,
+      a.wait_polls ? a.wait_polls : kChunkWaitPolls);
+  return serve_launched("tr_paged_attention");
+}
+
+int launch_attend_chunk(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
+  if (a.dtype == TR_F16)
+    return a.head_dim == 128 ? launch_chunk<__half, 128>(a, ws, stream)
+                             : launch_chunk<__half, 64>(a, ws, stream);
+  return a.head_dim == 128 ? launch_chunk<__nv_bfloat16, 128>(a, ws, stream)
+                           : launch_chunk<__nv_bfloat16, 64>(a, ws, stream);
+}
+
+}  // namespace trr

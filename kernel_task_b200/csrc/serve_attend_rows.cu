@@ -363,21 +363,41 @@ __global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_atte
       __syncthreads();
       writes = sh_last;
       if (writes) {
+        // eight partial results at a time: their loads are in flight together
         top = -INFINITY;
-        for (int64_t c = first_block; c <= last_block; ++c)
-          top = fmaxf(top, __ldcg(slot(c) + ROWS * D + orow));
-        const float all = top == -INFINITY ? 0.f : top;
         sum = 0.f;
 #pragma unroll
         for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
-        for (int64_t c = first_block; c <= last_block; ++c) {
-          const float* p = slot(c);
-          const float f = exp2_approx(__ldcg(p + ROWS * D + orow) - all);
-          sum += f * __ldcg(p + ROWS * D + ROWS + orow);
+        for (int64_t c0 = first_block; c0 <= last_block; c0 += 8) {
+          float pm[8], pl[8];
+          float4 pv[8][COLS / 4];
 #pragma unroll
-          for (int k = 0; k < COLS; k += 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + orow * D + ocol + k));
-            acc[k] += f * v.x, acc[k + 1] += f * v.y, acc[k + 2] += f * v.z, acc[k + 3] += f * v.w;
+          for (int j = 0; j < 8; ++j) {
+            const float* p = slot(min(c0 + j, last_block));
+            pm[j] = c0 + j <= last_block ? __ldcg(p + ROWS * D + orow) : -INFINITY;
+            pl[j] = __ldcg(p + ROWS * D + ROWS + orow);
+#pragma unroll
+            for (int k = 0; k < COLS / 4; ++k)
+              pv[j][k] = __ldcg(reinterpret_cast<const float4*>(p + orow * D + ocol) + k);
+          }
+          float all = top;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) all = fmaxf(all, pm[j]);
+          const float base = all == -INFINITY ? 0.f : all;
+          const float keep = exp2_approx(top - base);
+          top = all;
+          sum *= keep;
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) acc[c] *= keep;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float f = exp2_approx(pm[j] - base);
+            sum += f * pl[j];
+#pragma unroll
+            for (int k = 0; k < COLS / 4; ++k) {
+              acc[4 * k] += f * pv[j][k].x, acc[4 * k + 1] += f * pv[j][k].y;
+              acc[4 * k + 2] += f * pv[j][k].z, acc[4 * k + 3] += f * pv[j][k].w;
+            }
           }
         }
       }
@@ -411,13 +431,13 @@ static int64_t rows_max_items(const tr_attention& a, int rows) {
 }
 static int rows_grid() { return serve_sms() * 2; }
 
-size_t attend_partials_bytes() {
-  return (size_t)rows_grid() * 2 * partial_floats(16, 128) * sizeof(float);
+int64_t attend_rows_items(const tr_attention& a) { return rows_max_items(a, rows_of_tile(a)); }
+size_t attend_rows_partials(const tr_attention& a) {
+  return (size_t)rows_grid() * 2 * partial_floats(rows_of_tile(a), a.head_dim) * sizeof(float);
 }
-size_t attend_rows_counters(const tr_attention& a) { return rows_max_items(a, rows_of_tile(a)); }
 
 template <typename E, int D, int NT>
-static int launch_rows(const tr_attention& a, void* workspace, void* stream) {
+static int launch_rows(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
   constexpr int pipeline = kRowsWarps * kRowsStages * 2 * warp_keys<D>() * D * 2;
   constexpr int joined = kRowsWarps * 8 * NT * (D + 4) * 4;
   constexpr int smem = pipeline > joined ? pipeline : joined;
@@ -428,25 +448,24 @@ static int launch_rows(const tr_attention& a, void* workspace, void* stream) {
     set_error("tr_paged_attention: %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     return TR_ERR_CUDA;
   }
-  int* counters = reinterpret_cast<int*>(static_cast<char*>(workspace) + attend_partials_bytes());
   kernel<<<rows_grid(), kRowsThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-      a, counters, rows_max_items(a, 8 * NT), static_cast<float*>(workspace));
+      a, ws.counters, rows_max_items(a, 8 * NT), ws.partials);
   return serve_launched("tr_paged_attention");
 }
 
 template <typename E>
-static int launch_rows_type(const tr_attention& a, void* workspace, void* stream) {
+static int launch_rows_type(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
   const bool wide = rows_of_tile(a) == 16;
   if (a.head_dim == 128)
-    return wide ? launch_rows<E, 128, 2>(a, workspace, stream)
-                : launch_rows<E, 128, 1>(a, workspace, stream);
-  return wide ? launch_rows<E, 64, 2>(a, workspace, stream)
-              : launch_rows<E, 64, 1>(a, workspace, stream);
+    return wide ? launch_rows<E, 128, 2>(a, ws, stream)
+                : launch_rows<E, 128, 1>(a, ws, stream);
+  return wide ? launch_rows<E, 64, 2>(a, ws, stream)
+              : launch_rows<E, 64, 1>(a, ws, stream);
 }
 
-int launch_attend_rows(const tr_attention& a, void* workspace, void* stream) {
-  return a.dtype == TR_F16 ? launch_rows_type<__half>(a, workspace, stream)
-                           : launch_rows_type<__nv_bfloat16>(a, workspace, stream);
+int launch_attend_rows(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
+  return a.dtype == TR_F16 ? launch_rows_type<__half>(a, ws, stream)
+                           : launch_rows_type<__nv_bfloat16>(a, ws, stream);
 }
 
 }  // namespace trr

@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -157,22 +158,52 @@ void append_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pag
         "tr_append_kv");
 }
 
-// The attention's workspace: one buffer per device and stream, zeroed when it is made and left
-// ready by every call, so calls in one stream share it and calls in two streams do not meet in
-// it.  While the stream is being captured a call gets a buffer of its own, whose zeroing is
-// captured with it, because the graph may be replayed next to later calls on the stream.
+// The attention's workspace: one buffer per device and stream, its state zeroed when it is made
+// and left ready by every call, so calls in one stream share it and calls in two streams do not
+// meet in it.  While the stream is being captured a call gets a buffer of its own, whose zeroing
+// is captured with it, because the graph may be replayed next to later calls on the stream.
+at::Tensor new_workspace(int64_t bytes, const at::Tensor& like, cudaStream_t stream) {
+  at::Tensor ws = at::empty({bytes}, like.options().dtype(at::kByte));
+  check(tr_workspace_clear(ws.data_ptr(), TR_ATTENTION_STATE_BYTES, stream), "tr_workspace_clear");
+  return ws;
+}
+std::mutex workspaces_lock;
+std::map<std::pair<int, cudaStream_t>, at::Tensor>& workspaces() {
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
+  return *kept;
+}
 at::Tensor attention_workspace(int64_t bytes, const at::Tensor& like, cudaStream_t stream) {
-  const auto options = like.options().dtype(at::kByte);
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess)
     throw std::runtime_error("paged_attention: cudaStreamIsCapturing failed");
-  if (capture != cudaStreamCaptureStatusNone) return at::zeros({bytes}, options);
-  static std::mutex lock;
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
-  const std::lock_guard<std::mutex> hold(lock);
-  at::Tensor& ws = (*kept)[{like.get_device(), stream}];
-  if (!ws.defined() || ws.numel() < bytes) ws = at::zeros({bytes}, options);
+  if (capture != cudaStreamCaptureStatusNone) return new_workspace(bytes, like, stream);
+  const std::lock_guard<std::mutex> hold(workspaces_lock);
+  at::Tensor& ws = workspaces()[{like.get_device(), stream}];
+  if (!ws.defined() || ws.numel() < bytes) ws = new_workspace(bytes, like, stream);
   return ws;
+}
+
+// TRR_CHECK_STATUS=1: after every call outside a capture, read the status word (a stream
+// synchronisation) and raise if a bounded device-side wait gave up.  Debugging aid.
+bool checks_status() {
+  static const bool on = [] {
+    const char* v = std::getenv("TRR_CHECK_STATUS");
+    return v && v[0] == '1';
+  }();
+  return on;
+}
+void check_status(const at::Tensor& ws, const at::Tensor& like, cudaStream_t stream) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess ||
+      capture != cudaStreamCaptureStatusNone)
+    return;
+  int32_t status = TR_OK;
+  check(tr_workspace_status(ws.data_ptr(), ws.numel(), &status, 0, stream), "tr_workspace_status");
+  if (status == TR_OK) return;
+  const std::lock_guard<std::mutex> hold(workspaces_lock);
+  workspaces().erase({like.get_device(), stream});  // its counters are not valid any more
+  throw std::runtime_error(std::string("paged_attention: ") + tr_status_string(status) +
+                           " (the call's output is not valid)");
 }
 
 std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::Tensor& k_pages,
@@ -233,6 +264,7 @@ std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::
   if (bytes) ws = attention_workspace((int64_t)bytes, q, stream);
   check(tr_paged_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes ? ws.numel() : 0, stream),
         "tr_paged_attention");
+  if (bytes && checks_status()) check_status(ws, q, stream);
   if (!return_lse) return {out, c10::nullopt};
   return {out, lse};
 }
