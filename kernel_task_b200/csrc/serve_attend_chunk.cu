@@ -4,16 +4,18 @@
 // A row is one token and query head; the rows of a request over one kv head, token-major, are
 // cut into tiles of 256, so all the heads that share keys share their loads.  A tile is two
 // subtiles of 128 rows, each with its own scores S and output O in tensor memory:
-//     S = Q K^T   (128 x 128 keys, K-major operands in shared memory, 128-byte swizzle)
+//     S = Q K^T   (128 x 64 keys, K-major operands in shared memory, 128-byte swizzle)
 //     O += P V    (P from tensor memory, where it takes the place of S; V is read with its
 //                  head_dim contiguous, the MN-major form of the same layout)
+// Each subtile has two buffers of S, so the next 64 keys' scores are made while the softmax works
+// on these: with one buffer of 128 keys the chain scores - softmax - product ran at half the
+// products' rate.  64 wide is what two subtiles with a head_dim of 128 leave of 512 columns.
 // Warps 0-3 and 4-7 each hold a subtile's softmax, a thread per row: running maximum and sum in
 // registers, P rounded to the values' type.  O is rescaled only when a row's maximum grew by
 // more than 2^8 since the last time; P is then at most 256 and the fp32 sums keep their bits.
-// Warp 8 issues the products, alternating the subtiles so that one's softmax runs under the
-// other's products; warps 9 and 10 bring keys and values, 128 rows at a time, through a ring of
-// shared-memory slots with cp.async (zeros past the keys: a page's unused rows may hold
-// anything, and 0 * NaN would reach O).
+// Warp 8 issues the scores, warp 11 the products with V; warps 9 and 10 bring queries, keys and
+// values, 128 rows at a time, through a ring of shared-memory slots with cp.async (zeros past
+// the keys: a page's unused rows may hold anything, and 0 * NaN would reach O).
 //
 // Split.  An item is (request, row tile, kv head), a unit one block of 128 keys that the tile
 // sees; kItemUnits more stand in front of them for what an item costs besides (queries, the
@@ -32,18 +34,14 @@ namespace trr {
 
 constexpr int kBlockKeys = 128;
 constexpr int kSubRows = 128, kTileRows = 2 * kSubRows;
-constexpr int kChunkThreads = 11 * 32;
+constexpr int kChunkThreads = 12 * 32;
 constexpr int kMinChunkUnits = 6;  // units a grid block takes at least
 constexpr int kItemUnits = 3;
-constexpr unsigned kChunkWaitPolls = 1u << 21;
+constexpr unsigned kChunkWaitPolls = 1u << 16;  // of about 20 us
 
 template <int D>
 __host__ __device__ constexpr int ring_slots() {
   return D == 128 ? 5 : 8;
-}
-template <int D>
-__host__ __device__ constexpr int loads_in_flight() {
-  return D == 128 ? 2 : 4;
 }
 template <int D>
 __host__ __device__ constexpr int slot_bytes() {
@@ -88,6 +86,65 @@ __device__ __forceinline__ void umma_ts_one(uint32_t dtmem, uint32_t atmem, uint
       "r"(atmem), "l"(db), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
 }
 
+// ---- pairs of fp32
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// P of 32 keys from their scores: 2^(s scale - base), rounded in pairs to E; their sums added to
+// `sum`.
+template <typename E>
+__device__ __forceinline__ void probabilities(const uint32_t* s, uint64_t scale, uint64_t minus_base,
+                                              uint64_t (&sum)[2], uint32_t (&p)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float2 x = unpair(fma2(pair(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])),
+                                 scale, minus_base));
+    const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
+    sum[k & 1] = add2(sum[k & 1], pair(e0, e1));
+    p[k] = pack2<E>(e0, e1);
+  }
+}
+
+// Four 16-byte chunks of this lane's row become chunk lane & 3 of the four rows of its quad, so
+// that a warp's store covers 64 contiguous bytes of 8 rows instead of 16 bytes of 32.
+__device__ __forceinline__ uint4 swap4(uint4 v, int x) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, x), __shfl_xor_sync(0xffffffffu, v.y, x),
+                    __shfl_xor_sync(0xffffffffu, v.z, x), __shfl_xor_sync(0xffffffffu, v.w, x));
+}
+__device__ __forceinline__ void quad_transpose(uint4 (&c)[4]) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint4 got = swap4(odd ? c[i] : c[i + 1], 1);
+    if (odd) c[i] = got;
+    else c[i + 1] = got;
+  }
+  // now c[0], c[1]: chunk `odd` of the quad's even and odd row of this half; c[2], c[3]: 2 + odd
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 got = swap4(high ? c[i] : c[i + 2], 2);
+    if (high) c[i] = got;
+    else c[i + 2] = got;
+  }
+}
+
 // Keys and values of a slot: [head_dim / 64][128 rows][128 bytes], 16-byte chunks swizzled by
 // row & 7.  Values as the MN-major operand: 64-element column groups 16 KB apart, groups of 8
 // keys 1024 bytes apart.
@@ -98,22 +155,33 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t saddr) {
 
 // Walks the items of a contiguous run of units.
 struct ChunkItem {
-  int request, n, rows, tiles, tile, kvh, units;  // units: kItemUnits, then the blocks of keys
-  int64_t u0;     // first unit of the item
-  int64_t index;  // item number
+  int request, rows, tiles, tile, kvh;
+  int units;       // of the item: kItemUnits, then its blocks of keys
+  int see0, cap;   // token i of the request sees min(see0 + i, cap) keys (none if negative)
+  int64_t token0;  // the request's first token
+  int64_t u0;      // first unit of the item
+  int64_t index;   // item number
 };
-__device__ __forceinline__ int tile_units(const tr_attention& a, int r, int n, int g, int tile,
-                                          int rows) {
-  const int last = min((tile + 1) * kTileRows, rows) - 1;
-  return max((visible(a, r, n, last / g) + kBlockKeys - 1) / kBlockKeys, 1) + kItemUnits;
+__device__ __forceinline__ int keys_of_token(const ChunkItem& it, int i) {
+  return max(min(it.see0 + i, it.cap), 0);
+}
+// keys that the last row of the tile sees
+__device__ __forceinline__ int keys_of_tile(const ChunkItem& it, int g, int tile) {
+  return keys_of_token(it, (min((tile + 1) * kTileRows, it.rows) - 1) / g);
+}
+__device__ __forceinline__ int tile_units(const ChunkItem& it, int g, int tile) {
+  return max((keys_of_tile(it, g, tile) + kBlockKeys - 1) / kBlockKeys, 1) + kItemUnits;
 }
 __device__ __forceinline__ void open_request(const tr_attention& a, int g, ChunkItem& it, int r) {
+  const int n = brought(a, r);
   it.request = r;
-  it.n = brought(a, r);
-  it.rows = it.n * g;
+  it.rows = n * g;
   it.tiles = (it.rows + kTileRows - 1) / kTileRows;
   it.tile = it.kvh = 0;
-  it.units = it.tiles ? tile_units(a, r, it.n, g, 0, it.rows) : 0;
+  it.cap = cached(a, r);
+  it.see0 = (int)max((int64_t)a.lens[r] - n + 1, -(int64_t)(1 << 30));
+  it.token0 = max((int64_t)a.starts[r], (int64_t)0);
+  it.units = it.tiles ? tile_units(it, g, 0) : 0;
 }
 __device__ __forceinline__ void next_item(const tr_attention& a, int g, ChunkItem& it) {
   it.u0 += it.units;
@@ -121,7 +189,7 @@ __device__ __forceinline__ void next_item(const tr_attention& a, int g, ChunkIte
   if (++it.kvh < a.kv_heads) return;
   it.kvh = 0;
   if (++it.tile < it.tiles) {
-    it.units = tile_units(a, it.request, it.n, g, it.tile, it.rows);
+    it.units = tile_units(it, g, it.tile);
     return;
   }
   while (it.request + 1 < (int)a.requests) {
@@ -140,23 +208,24 @@ __device__ __forceinline__ Segment take(const ChunkItem& it, int64_t& u, int64_t
 }
 
 enum {
-  B_FULL = 0,        // [8] a slot's rows have arrived
-  B_EMPTY = 8,       // [8] the products have read a slot
-  B_QUERY = 16,      // [2] a subtile's queries are in shared memory
-  B_SCORES = 18,     // [2] S is in tensor memory
-  B_PROBS = 20,      // [2] P has taken its place, O is rescaled
-  B_OUT = 22,        // [2] O is complete
-  B_LEFT = 24,       // [2] a subtile's partial result is written
-  B_JOIN = 26,       // [2] whether this block joins the item is known
-  B_DRAIN = 28,
-  B_COUNT = 29
+  B_FULL = 0,    // [8] a slot's rows have arrived (the copies arrive by themselves)
+  B_EMPTY = 8,   // [8] the products have read a slot
+  B_QUERY = 16,  // the tile's queries are in shared memory
+  B_QFREE = 17,  // the item's last scores are made: the queries' place is free
+  B_SCORES = 18, // [2][2] a subtile's S of the first or last 64 keys is in tensor memory
+  B_PROBS = 22,  // [2][2] P has taken its place, O is rescaled
+  B_PRODUCT = 26, // [2][2] their P V is added to the subtile's O
+  B_LEFT = 30,   // [2] a subtile's partial result is written
+  B_JOIN = 32,   // [2] whether this block joins the item is known
+  B_DRAIN = 34,  // [2] an issuing warp's last products
+  B_COUNT = 36
 };
 
 template <typename E, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attend_chunk_kernel(const tr_attention a, int* status, int* counters, int64_t max_items,
                         float* partials, unsigned wait_polls) {
-  constexpr int NS = ring_slots<D>(), FLIGHT = loads_in_flight<D>();
+  constexpr int NS = ring_slots<D>();
   constexpr int QBYTES = kSubRows * D * 2, SLOT = slot_bytes<D>(), CPR = D / 8;
   constexpr int64_t PARTIAL = (int64_t)kTileRows * (D + 2);
   extern __shared__ uint8_t smem_raw[];
@@ -180,7 +249,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     open_request(a, g, it, r);
     my_items += (int64_t)it.tiles * a.kv_heads;
     for (int t = 0; t < it.tiles; ++t)
-      my_units += (int64_t)tile_units(a, r, it.n, g, t, it.rows) * a.kv_heads;
+      my_units += (int64_t)tile_units(it, g, t) * a.kv_heads;
   }
   int64_t U, all_items;
   const int64_t through = block_scan_inclusive(my_units, scan_part, U);
@@ -197,7 +266,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       open_request(a, g, it, r);
       int64_t units = 0;
       for (; it.tile < it.tiles; ++it.tile) {
-        it.units = tile_units(a, r, it.n, g, it.tile, it.rows);
+        it.units = tile_units(it, g, it.tile);
         units = (int64_t)it.units * a.kv_heads;
         if (u_begin < it.u0 + units) break;
         it.u0 += units;
@@ -221,13 +290,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (warp == 9) {
-    if (lane < B_COUNT) {
+    for (int i = lane; i < B_COUNT; i += 32) {
       int count = 1;
-      if (lane < B_EMPTY) count = 2;  // the two loading warps
-      if (lane == B_QUERY || lane == B_QUERY + 1 || lane == B_PROBS || lane == B_PROBS + 1 ||
-          lane == B_LEFT || lane == B_LEFT + 1)
+      if (i < B_EMPTY || i == B_QUERY) count = 64;  // the threads of the two loading warps
+      if ((i >= B_PROBS && i < B_PRODUCT) || i == B_LEFT || i == B_LEFT + 1)
         count = 4;  // the subtile's four warps
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar(lane)), "r"(count)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar(i)), "r"(count)
                    : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -241,8 +309,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t qbase = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t ring = qbase + 2 * QBYTES;
   volatile int* abort = &sh_abort;
+  // Bounded wait of a whole warp.  try_wait suspends the warp, up to some 20 us at a time, which
+  // leaves the issue slots to the softmax (polling: 4 % faster over long contexts with a head_dim
+  // of 128, 9 % slower with 64 and over short prompts).
   const auto wait = [&](int b, uint32_t parity) {
-    return warp_wait(bar(b), parity, abort, wait_polls);
+    bool ok = true;
+    for (unsigned i = 0; ok && !mbar_try(bar(b), parity); ++i) {
+      if (*abort) ok = false;
+      if (i >= wait_polls) {
+        *abort = 1;
+        ok = false;
+      }
+    }
+    return (bool)__all_sync(0xffffffffu, ok);
   };
   ChunkItem it = first_item;
   const int page_shift = 31 - __clz(a.page_size);
@@ -253,7 +332,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + t * 128 + lanes, o_tmem = tmem + 256 + t * D + lanes;
     const float scale2 = a.scale * kLog2e;
-    uint32_t uses = 0, scores = 0, lefts = 0;  // completed phases of this subtile's barriers
+    // phases so far: blocks of keys (B_SCORES, B_PROBS, B_PRODUCT), partial results
+    uint32_t blocks = 0, lefts = 0;
     for (int64_t u = u_begin; u < u_end; next_item(a, g, it)) {
       const Segment seg = take(it, u, u_end);
       const int b_first = seg.first, b_last = seg.last;
@@ -263,53 +343,48 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (rows_here <= 0) continue;  // the item has one subtile
       const bool live = row < rows_here;
       const int i = (row0 + row) / g, h = it.kvh * g + (row0 + row - i * g);
-      const int64_t token = (int64_t)max(a.starts[it.request], 0) + i;
-      const int limit = live ? visible(a, it.request, it.n, i) : 0;
+      const int limit = live ? keys_of_token(it, i) : 0;
       const bool warp_live = (warp & 3) * 32 < rows_here;
-
-      // queries, zeros past the rows
-      {
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) +
-                                                        token * a.q_token_stride +
-                                                        h * a.q_head_stride);
-        uint8_t* dst = smem_raw + (qbase - smem_u32(smem_raw)) + t * QBYTES + row * 128;
-#pragma unroll
-        for (int c = 0; c < CPR; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kSubRows * 128) + (((c & 7) ^ (row & 7)) << 4)) =
-              live ? q[c] : make_uint4(0, 0, 0, 0);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_QUERY + t));
-      }
 
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int b = b_first; b < b_last; ++b) {
-        if (!(ok = wait(B_SCORES + t, scores & 1))) break;
-        ++scores;
+      for (int n = 2 * b_first; n < 2 * b_last; ++n) {  // 64 keys at a time
+        const int half = n & 1;
+        const uint32_t s_half = s_tmem + half * 64;
+        if (!(ok = wait(B_SCORES + 2 * t + half, blocks & 1))) break;
         tc_fence_after();
         if (warp_live) {
-          uint32_t s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            tmem_ld<32>(s_tmem + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+          uint32_t s[64];
+          tmem_ld<32>(s_half, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+          tmem_ld<32>(s_half + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
           tmem_wait_ld();
-          const int seen = limit - b * kBlockKeys;
-          if (__any_sync(0xffffffffu, seen < kBlockKeys)) {
+          const int seen = limit - n * 64;
+          if (__any_sync(0xffffffffu, seen < 64)) {
 #pragma unroll
-            for (int k = 0; k < 128; ++k) s[k] = k < seen ? s[k] : __float_as_uint(-INFINITY);
+            for (int k = 0; k < 64; ++k) s[k] = k < seen ? s[k] : __float_as_uint(-INFINITY);
           }
-          float top = __uint_as_float(s[0]);
+          float tops[4];
 #pragma unroll
-          for (int k = 1; k < 128; ++k) top = fmaxf(top, __uint_as_float(s[k]));
-          top *= scale2;
+          for (int k = 0; k < 4; ++k) tops[k] = __uint_as_float(s[k]);
+#pragma unroll
+          for (int k = 4; k < 60; k += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tops[j] = fmaxf(fmaxf(tops[j], __uint_as_float(s[k + j])), __uint_as_float(s[k + 4 + j]));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tops[j] = fmaxf(tops[j], __uint_as_float(s[60 + j]));
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale2;
           // a new base where the old one would let P pass 2^8
           const bool rise = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
           if (__any_sync(0xffffffffu, rise)) {
             const float keep = !rise ? 1.f : m == -INFINITY ? 0.f : exp2_approx(m - top);
             if (rise) m = top;
             l *= keep;
-            if (b > b_first) {
+            if (n > 2 * b_first) {
+              // O holds still once the last 64 keys' product is added; the one before is
+              // already, since these scores came after it
+              if (!(ok = wait(B_PRODUCT + 2 * t + 1 - half, (blocks + half - 1) & 1))) break;
+              tc_fence_after();
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
@@ -322,27 +397,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
           }
           const float base = m == -INFINITY ? 0.f : m;
-          float sum = 0.f;
+          const uint64_t scales = pair(scale2, scale2), minus_base = pair(-base, -base);
+          uint64_t sum[2] = {0, 0};  // pairs of zeros
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float p0 = exp2_approx(fmaf(__uint_as_float(s[c * 32 + 2 * k]), scale2, -base));
-              const float p1 = exp2_approx(fmaf(__uint_as_float(s[c * 32 + 2 * k + 1]), scale2, -base));
-              sum += p0 + p1;
-              p[k] = pack2<E>(p0, p1);
-            }
-            tmem_st16(s_tmem + c * 16, p);
+            probabilities<E>(s + c * 32, scales, minus_base, sum, p);
+            tmem_st16(s_half + c * 16, p);
           }
-          l += sum;
+          const float2 all = unpair(add2(sum[0], sum[1]));
+          l += all.x + all.y;
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_PROBS + t));
+        if (lane == 0) mbar_arrive(bar(B_PROBS + 2 * t + half));
+        blocks += half;
       }
-      if (!ok || !wait(B_OUT + t, uses & 1)) break;
+      if (!ok || !wait(B_PRODUCT + 2 * t, (blocks - 1) & 1) ||
+          !wait(B_PRODUCT + 2 * t + 1, (blocks - 1) & 1))
+        break;
       tc_fence_after();
 
       const bool shared_item = b_last - b_first < it.units - kItemUnits;
@@ -351,6 +425,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int64_t last_block = ((it.u0 + it.units) * G - 1) / U;
       const auto slot = [&](int64_t c) {
         return partials + (2 * c + (U * c / G < it.u0 ? 1 : 0)) * PARTIAL;
+      };
+      // the quad's four rows: element offset of each in out, or -1
+      const int64_t out_row = ((it.token0 + i) * a.heads + h);
+      int64_t quad_row[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        quad_row[k] = __shfl_sync(0xffffffffu, live ? out_row : -1, (lane & ~3) + k);
+      const auto store4 = [&](int col, uint4 (&c)[4]) {  // 32 columns from col
+        quad_transpose(c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (quad_row[k] >= 0)
+            *reinterpret_cast<uint4*>(static_cast<E*>(a.out) + quad_row[k] * D + col +
+                                      (lane & 3) * 8) = c[k];
       };
       bool writes = true;
       if (shared_item) {
@@ -398,156 +486,171 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         writes = sh_join[t];
         __threadfence();
         if (writes && warp_live) {
-          if (live) {
-            // half the columns at a time: 16 loads of a part in flight
-            const float* maxima = partials + (int64_t)kTileRows * D + at;
-            const float* sums = maxima + kTileRows;
-            const auto part = [&](int64_t c) { return slot(c) - partials; };
-            float top = -INFINITY;
+          // half the columns at a time: 16 loads of a part in flight (rows past the tile's
+          // read what the slot holds and store nothing)
+          const float* maxima = partials + (int64_t)kTileRows * D + at;
+          const float* sums = maxima + kTileRows;
+          const auto part = [&](int64_t c) { return slot(c) - partials; };
+          float top = -INFINITY;
 #pragma unroll 4
-            for (int64_t c = first_block; c <= last_block; ++c)
-              top = fmaxf(top, __ldcg(maxima + part(c)));
-            const float base = top == -INFINITY ? 0.f : top;
-            float sum = 0.f;
+          for (int64_t c = first_block; c <= last_block; ++c)
+            top = fmaxf(top, __ldcg(maxima + part(c)));
+          const float base = top == -INFINITY ? 0.f : top;
+          float sum = 0.f;
 #pragma unroll 4
-            for (int64_t c = first_block; c <= last_block; ++c)
-              sum += exp2_approx(__ldcg(maxima + part(c)) - base) * __ldcg(sums + part(c));
-            m = top;
-            l = sum;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-            E* out = static_cast<E*>(a.out) + (token * a.heads + h) * D;
+          for (int64_t c = first_block; c <= last_block; ++c)
+            sum += exp2_approx(__ldcg(maxima + part(c)) - base) * __ldcg(sums + part(c));
+          m = top;
+          l = sum;
+          const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 64) {
-              float acc[64];
+          for (int c0 = 0; c0 < D; c0 += 64) {
+            float acc[64];
 #pragma unroll
-              for (int k = 0; k < 64; ++k) acc[k] = 0.f;
+            for (int k = 0; k < 64; ++k) acc[k] = 0.f;
 #pragma unroll 1
-              for (int64_t c = first_block; c <= last_block; ++c) {
-                const float f = exp2_approx(__ldcg(maxima + part(c)) - base);
-                float4 v[16];
+            for (int64_t c = first_block; c <= last_block; ++c) {
+              const float f = exp2_approx(__ldcg(maxima + part(c)) - base);
+              float4 v[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  v[k] = __ldcg(reinterpret_cast<const float4*>(slot(c)) +
-                                (c0 / 4 + k) * kTileRows + at);
+              for (int k = 0; k < 16; ++k)
+                v[k] = __ldcg(reinterpret_cast<const float4*>(slot(c)) + (c0 / 4 + k) * kTileRows + at);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  acc[4 * k] += f * v[k].x, acc[4 * k + 1] += f * v[k].y;
-                  acc[4 * k + 2] += f * v[k].z, acc[4 * k + 3] += f * v[k].w;
-                }
+              for (int k = 0; k < 16; ++k) {
+                acc[4 * k] += f * v[k].x, acc[4 * k + 1] += f * v[k].y;
+                acc[4 * k + 2] += f * v[k].z, acc[4 * k + 3] += f * v[k].w;
               }
+            }
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                float v[8];
+            for (int k = 0; k < 64; k += 32) {
+              uint4 c[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = acc[8 * k + j] * inv;
-                store8<E>(out + c0 + k * 8, v);
-              }
+              for (int j = 0; j < 4; ++j)
+                c[j] = make_uint4(pack2<E>(acc[k + 8 * j] * inv, acc[k + 8 * j + 1] * inv),
+                                  pack2<E>(acc[k + 8 * j + 2] * inv, acc[k + 8 * j + 3] * inv),
+                                  pack2<E>(acc[k + 8 * j + 4] * inv, acc[k + 8 * j + 5] * inv),
+                                  pack2<E>(acc[k + 8 * j + 6] * inv, acc[k + 8 * j + 7] * inv));
+              store4(c0 + k, c);
             }
           }
         }
       } else if (warp_live) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        E* out = static_cast<E*>(a.out) + (token * a.heads + h) * D;
+        const float inv = m > -INFINITY ? 1.f / l : 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld<16>(o_tmem + c * 16, o);
+        for (int k = 0; k < D; k += 32) {
+          uint32_t o[32];
+          tmem_ld<32>(o_tmem + k, o);
           tmem_wait_ld();
-          if (live) {
+          uint4 c[4];
+          const auto two = [&](int n) {
+            return pack2<E>(__uint_as_float(o[n]) * inv, __uint_as_float(o[n + 1]) * inv);
+          };
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float v[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[8 * k + j]) * inv;
-              store8<E>(out + c * 16 + k * 8, v);
-            }
-          }
+          for (int j = 0; j < 4; ++j)
+            c[j] = make_uint4(two(8 * j), two(8 * j + 2), two(8 * j + 4), two(8 * j + 6));
+          store4(k, c);
         }
       }
       if (writes && live && a.lse)
-        a.lse[token * a.heads + h] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-      ++uses;
-      tc_fence_before();  // O and Q are free for the next item once B_QUERY and B_PROBS arrive
+        a.lse[out_row] = m > -INFINITY ? (m + log2f(l)) * kLn2 : -INFINITY;
+      tc_fence_before();  // O is free for the next item once its B_PROBS arrive
     }
   } else if (warp == 8) {
-    // ---- products
-    constexpr uint32_t idesc_s = umma_idesc<E>(kSubRows, kBlockKeys);
-    constexpr uint32_t idesc_o = umma_idesc<E>(kSubRows, D) | 1u << 16;  // values: MN-major
-    uint32_t x = 0;                     // slots taken so far
-    uint32_t items_done[2] = {0, 0}, probs[2] = {0, 0};
-    const auto scores = [&](int t, uint32_t slot) {
-      const uint32_t q = qbase + t * QBYTES, k = ring + slot * SLOT;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t in = (ks & 3) * 32;
-        umma_one(tmem + t * 128, desc_sw128(q + (ks >> 2) * (kSubRows * 128) + in),
-                 desc_sw128(k + (ks >> 2) * (kBlockKeys * 128) + in), idesc_s, ks > 0);
-      }
-      commit_one(bar(B_SCORES + t));
-    };
+    // ---- scores.  Each kind of product has a warp of its own: a wait takes some 200 cycles even
+    // when it is over, and the queue of products is shorter than that
+    constexpr uint32_t idesc_s = umma_idesc<E>(kSubRows, 64);
+    uint32_t items_done = 0, x = 0, blocks[2] = {0, 0};  // slots taken; blocks of a subtile
     bool ok = true;
     for (int64_t u = u_begin; ok && u < u_end; next_item(a, g, it)) {
       const Segment seg = take(it, u, u_end);
       const int b_first = seg.first, b_last = seg.last;
       if (b_first == b_last) continue;  // only the units in front
       const int subs = it.rows - it.tile * kTileRows > kSubRows ? 2 : 1;
-      uint32_t slot_k = x % NS;
-      ok = wait(B_FULL + slot_k, (x / NS) & 1);
-      for (int t = 0; ok && t < subs; ++t) {
-        if (!(ok = wait(B_QUERY + t, items_done[t] & 1))) break;
-        ++items_done[t];
-        tc_fence_after();
-        scores(t, slot_k);
-      }
-      if (!ok) break;
-      commit_one(bar(B_EMPTY + slot_k));
-      ++x;
+      if (!(ok = wait(B_QUERY, items_done & 1))) break;
+      ++items_done;
       for (int b = b_first; ok && b < b_last; ++b) {
-        const uint32_t slot_v = x % NS, next_k = (x + 1) % NS;
-        const bool more = b + 1 < b_last;
-        if (!(ok = wait(B_FULL + slot_v, (x / NS) & 1))) break;
-        for (int t = 0; t < subs; ++t) {
-          if (!(ok = wait(B_PROBS + t, probs[t] & 1))) break;
-          ++probs[t];
-          tc_fence_after();
+        const uint32_t slot = x % NS, keys = ring + slot * SLOT;
+        if (!(ok = wait(B_FULL + slot, (x / NS) & 1))) break;
+        fence_async_smem();  // the copies were ordinary writes; the products read by the async proxy
+        tc_fence_after();
+        for (int half = 0; ok && half < 2; ++half) {
+          for (int t = 0; t < subs; ++t) {
+            // P of the block before has been read from this half
+            if (blocks[t] && !(ok = wait(B_PRODUCT + 2 * t + half, (blocks[t] - 1) & 1))) break;
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < kBlockKeys / 16; ++ks)
-            umma_ts_one(tmem + 256 + t * D, tmem + t * 128 + ks * 8,
-                        desc_values(ring + slot_v * SLOT + ks * 2048), idesc_o,
-                        b > b_first || ks > 0);
-          if (more) {
-            if (t == 0 && !(ok = wait(B_FULL + next_k, ((x + 1) / NS) & 1))) break;
-            scores(t, next_k);
-          } else {
-            commit_one(bar(B_OUT + t));
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint32_t in = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+              umma_one(tmem + t * 128 + half * 64, desc_sw128(qbase + t * QBYTES + in),
+                       desc_sw128(keys + half * (64 * 128) + in), idesc_s, ks > 0);
+            }
+            commit_one(bar(B_SCORES + 2 * t + half));
           }
         }
         if (!ok) break;
-        commit_one(bar(B_EMPTY + slot_v));
-        if (more) commit_one(bar(B_EMPTY + next_k));
-        x += more ? 2 : 1;
+        for (int t = 0; t < subs; ++t) ++blocks[t];
+        commit_one(bar(B_EMPTY + slot));
+        if (b + 1 == b_last) commit_one(bar(B_QFREE));
+        x += 2;
       }
     }
-    // whatever was issued has to end before tensor memory is freed
-    commit_one(bar(B_DRAIN));
+    commit_one(bar(B_DRAIN));  // whatever was issued has to end before tensor memory is freed
     mbar_drain_spin(bar(B_DRAIN), 0);
-  } else {
-    // ---- loads: warp w brings rows 64 w .. 64 w + 63 of every block of keys and of values
-    const int w = warp - 9;
-    uint32_t x = 0;
+  } else if (warp == 11) {
+    // ---- products with the values
+    constexpr uint32_t idesc_o = umma_idesc<E>(kSubRows, D) | 1u << 16;  // values: MN-major
+    uint32_t x = 1, blocks[2] = {0, 0};
     bool ok = true;
-    const uint4* pools[2] = {static_cast<const uint4*>(a.k_pages),
-                             static_cast<const uint4*>(a.v_pages)};
-    // a lane's destination inside a slot: chunk c of row 64 w + lane / CPR, and the rows below it
-    const int c = lane % CPR, sub = lane / CPR;
-    constexpr int RPI = 32 / CPR;  // rows an instruction of the warp covers
     for (int64_t u = u_begin; ok && u < u_end; next_item(a, g, it)) {
       const Segment seg = take(it, u, u_end);
       const int b_first = seg.first, b_last = seg.last;
-      if (b_first == b_last) continue;  // only the units in front
-      const int rows_tile = min(it.rows - it.tile * kTileRows, kTileRows);
-      const int keys_end =
-          max(visible(a, it.request, it.n, (it.tile * kTileRows + rows_tile - 1) / g), 0);
+      if (b_first == b_last) continue;
+      const int subs = it.rows - it.tile * kTileRows > kSubRows ? 2 : 1;
+      for (int b = b_first; ok && b < b_last; ++b) {
+        const uint32_t slot = x % NS, values = ring + slot * SLOT;
+        if (!(ok = wait(B_FULL + slot, (x / NS) & 1))) break;
+        fence_async_smem();
+        for (int half = 0; ok && half < 2; ++half) {
+          for (int t = 0; t < subs; ++t) {
+            if (!(ok = wait(B_PROBS + 2 * t + half, blocks[t] & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              umma_ts_one(tmem + 256 + t * D, tmem + t * 128 + half * 64 + ks * 8,
+                          desc_values(values + (half * 4 + ks) * 2048), idesc_o,
+                          b > b_first || half > 0 || ks > 0);
+            commit_one(bar(B_PRODUCT + 2 * t + half));
+          }
+        }
+        if (!ok) break;
+        for (int t = 0; t < subs; ++t) ++blocks[t];
+        commit_one(bar(B_EMPTY + slot));
+        x += 2;
+      }
+    }
+    commit_one(bar(B_DRAIN + 1));
+    mbar_drain_spin(bar(B_DRAIN + 1), 0);
+  } else {
+    // ---- loads: warp w brings rows 64 w .. 64 w + 63 of every block of keys and of values, and
+    // of both subtiles' queries
+    const int w = warp - 9;
+    uint32_t x = 0, items_done = 0;
+    bool ok = true;
+    // a lane's part: chunk c of row `sub` and of every RPI-th row after it
+    const int c = lane % CPR, sub = lane / CPR;
+    constexpr int RPI = 32 / CPR;
+    const auto at_row = [&](int rr) {  // offset of the chunk in a [head_dim / 64][rows][128 B] array
+      return rr * 128 + (((c & 7) ^ (rr & 7)) << 4) + (c >> 3) * (128 * 128);
+    };
+    // arrives on `b` when this thread's copies so far are in shared memory
+    const auto hand_over = [&](int b) {
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar(b)) : "memory");
+    };
+    for (int64_t u = u_begin; ok && u < u_end; next_item(a, g, it)) {
+      const Segment seg = take(it, u, u_end);
+      const int b_first = seg.first, b_last = seg.last;
+      if (b_first == b_last) continue;
+      const int keys_end = keys_of_tile(it, g, it.tile);
       const int32_t* table = a.tables + it.request * a.table_stride;
       // pool rows of keys 64 w + lane and + 32 of block b; ~0u past the keys and for bad pages
       uint32_t rows[2], next[2];
@@ -557,47 +660,63 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int key = b * kBlockKeys + w * 64 + j * 32 + lane;
           const int id = b < b_last && key < keys_end ? table[key >> page_shift] : -1;
           r[j] = id >= 0 && id < a.pages
-                     ? (uint32_t)((id * a.kv_heads + it.kvh) * (int64_t)a.page_size +
+                     ? (uint32_t)((id * (int64_t)a.kv_heads + it.kvh) * a.page_size +
                                   (key & (a.page_size - 1)))
                      : ~0u;
         }
       };
+      const auto load_rows = [&](const uint4* pool) {
+        const uint32_t slot = x % NS;
+        if (x >= NS && !(ok = wait(B_EMPTY + slot, (x / NS - 1) & 1))) return;
+        const uint32_t dst = ring + slot * SLOT + w * 64 * 128;
+#pragma unroll
+        for (int i = 0; i < 64 / RPI; ++i) {
+          const int rr = i * RPI + sub;
+          const uint32_t r = __shfl_sync(0xffffffffu, rows[i * RPI / 32], rr & 31);
+          const bool held = r != ~0u;
+          copy16_async(dst + at_row(rr), pool + (uint64_t)(held ? r : 0u) * CPR + c, held);
+        }
+        hand_over(B_FULL + slot);
+        ++x;
+      };
       find(b_first, rows);
       for (int b = b_first; ok && b < b_last; ++b) {
-        find(b + 1, next);
+        load_rows(static_cast<const uint4*>(a.k_pages));
+        if (!ok) break;
+        if (b == b_first) {
+          // the queries, once the last item's are read
+          if (items_done && !(ok = wait(B_QFREE, (items_done - 1) & 1))) break;
 #pragma unroll 1
-        for (int which = 0; which < 2; ++which) {
-          if (x >= FLIGHT) {  // the oldest load in flight has arrived: hand it over
-            copies_wait<FLIGHT - 1>();
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_FULL + (x - FLIGHT) % NS));
-          }
-          const uint32_t slot = x % NS;
-          if (x >= NS && !(ok = wait(B_EMPTY + slot, (x / NS - 1) & 1))) break;
-          const uint32_t dst = ring + slot * SLOT + w * 64 * 128 + (c >> 3) * (kBlockKeys * 128);
-          const uint4* pool = pools[which];
+          for (int t = 0; t < 2; ++t) {
+            // element offsets of rows 64 w + lane and + 32 of the subtile; -1 past the rows
+            int64_t from[2];
 #pragma unroll
-          for (int i = 0; i < 64 / RPI; ++i) {
-            const int rr = i * RPI + sub;
-            const uint32_t r = __shfl_sync(0xffffffffu, rows[i * RPI / 32], rr & 31);
-            const bool held = r != ~0u;
-            copy16_async(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4),
-                         pool + (uint64_t)(held ? r : 0u) * CPR + c, held);
+            for (int j = 0; j < 2; ++j) {
+              const int row = it.tile * kTileRows + t * kSubRows + w * 64 + j * 32 + lane;
+              const int i = row / g;
+              from[j] = row < it.rows ? (it.token0 + i) * a.q_token_stride +
+                                            (it.kvh * g + row - i * g) * a.q_head_stride
+                                      : -1;
+            }
+            const uint32_t dst = qbase + t * QBYTES + w * 64 * 128;
+#pragma unroll
+            for (int i = 0; i < 64 / RPI; ++i) {
+              const int rr = i * RPI + sub;
+              const int64_t f = __shfl_sync(0xffffffffu, from[i * RPI / 32], rr & 31);
+              copy16_async(dst + at_row(rr), static_cast<const E*>(a.q) + (f < 0 ? 0 : f) + c * 8,
+                           f >= 0);
+            }
           }
-          copies_commit();
-          ++x;
+          hand_over(B_QUERY);
+          ++items_done;
         }
+        find(b + 1, next);
+        load_rows(static_cast<const uint4*>(a.v_pages));
         rows[0] = next[0];
         rows[1] = next[1];
       }
     }
-    copies_wait<0>();
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0 && ok)
-      for (uint32_t i = x > FLIGHT ? x - FLIGHT : 0; i < x; ++i) mbar_arrive(bar(B_FULL + i % NS));
-    __syncwarp();
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
   }
 
   tc_fence_before();
