@@ -31,12 +31,6 @@ __device__ __forceinline__ int visible(const tr_attention& a, int r, int n, int 
   return (int)min((int64_t)a.lens[r] - n + i + 1, (int64_t)cached(a, r));
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 16 bytes global -> shared, asynchronously; zeros when !held (src is then not read)
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool held) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
@@ -49,7 +43,7 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
 
 // Zeros and -inf for the tokens outside [starts[0], starts[requests]); `thread` of `threads`.
 template <typename E>

@@ -229,39 +229,50 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   }
 }
 
-// ---- one cluster per row, the row's t in shared memory ------------------------------------
+// ---- one cluster per row, the row in shared memory -----------------------------------------
 //
-// Every block of the cluster holds a contiguous slice of t, so the logits are read once.  A
-// histogram of (greatest - t) in 1024 steps of 1/32, summed over the cluster, says down to which
-// step the limits reach.  Where that leaves at most kCandidates tokens (a top_k of some hundred, or
-// a top_p that the likeliest tokens reach) these are gathered, ranked, and all limits applied
-// to the ranked list; noise is then read for them alone.  Else each limit's cut is narrowed down by
-// further histograms over the steps that can hold it (for a mass: between the bounds that the
-// steps' edges give, with the exact mass above them) until few enough tokens or a single value is
-// left, and what is below the cut is struck out of the slices.
+// Every block of the cluster holds a contiguous slice of the logits, so they are read once.  The
+// order of t = logit / temperature is the logits' own, so maxima, histograms and cuts work on
+// the logits; t itself (an exact division) is made for the tokens that reach the final choice.
+//
+// The limits mostly leave few tokens.  Each thread's greatest logit goes into a histogram of 1024
+// steps below the greatest (1/32 of t each), summed over the cluster: these are some of the
+// tokens, so where they alone reach top_k, or top_p of the mass, all tokens kept lie in the steps
+// down to there.  They are gathered, ranked, and all limits applied to the ranked list; noise is
+// read for them alone.  Where they do not reach, or are over kCandidates, all logits are
+// counted, and each limit's cut is narrowed down by further histograms over the steps that can
+// hold it (for a mass: between the bounds that the steps' edges give, with the exact mass above
+// them) until few enough tokens or a single value is left; what is below the cut is struck out.
 // All sums run in an order fixed by the row alone.
 constexpr int kSliceThreads = 512;
 constexpr int kBins = 1024;
 constexpr float kBinsPerUnit = 32.f;
 constexpr int kCandidates = 512;
-constexpr int kMaxSlice = 52000;  // fp32 values of a block: 208 KB
+constexpr int kSliceBytes = 65536;     // of a block where the rows fill the GPU: three blocks an SM
+constexpr int kMaxSliceBytes = 200000;
 
 struct RowSums {  // one value or two per block of the cluster, in every block
   double v[2][8][2];
 };
 
 template <typename L>
+__device__ __forceinline__ L not_nan(L x) {
+  return to_f32<L>(x) == to_f32<L>(x) ? x : from_f32<L>(-INFINITY);
+}
+
+template <typename L>
 __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const SampleArgs a,
-                                                                     int slice_size) {
-  extern __shared__ float t_s[];
+                                                                        int slice_size) {
+  constexpr int W = 16 / sizeof(L);  // elements of a 16-byte load
+  extern __shared__ uint4 slice_raw[];
   __shared__ uint32_t hist[kBins];   // this block's, then the cluster's
   __shared__ uint32_t total[kBins];  // of block 0: the cluster's
   __shared__ RowSums sums;
-  __shared__ float cand_t[kCandidates], rank_t[kCandidates];
-  __shared__ int cand_i[kCandidates], rank_i[kCandidates];
+  __shared__ float own_l[kCandidates], cand_l[kCandidates];  // this block's; block 0: all
+  __shared__ int own_i[kCandidates], cand_i[kCandidates];
   __shared__ Best part[32], cluster_best[8];
   __shared__ double dpart[32];
-  __shared__ float fpart[32], cluster_t[8];
+  __shared__ float fpart[32], cluster_l[8];
   __shared__ int ipart[32];
   __shared__ int sh_count, sh_bin[2], sh_ties;
   __shared__ float sh_cut;
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   const float least_weight = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
 
   int turn = 0;
-  // Combines x (and y) over the cluster with `op`, in rank order; also a cluster barrier.
+  // Combines x and y over the cluster with `op`, in rank order; also a cluster barrier.
   const auto over_cluster = [&](double x, double y, auto op) {
     double(*box)[2] = sums.v[turn & 1];
     if (tid < ranks) {
@@ -319,31 +330,52 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
     return v;
   };
 
-  // ---- the slice: t, with NaN as -inf and -0 as 0; the greatest
+  // ---- the slice, NaN as -inf, in 16-byte groups from its first element on.  Where the row does
+  // not start on 16 bytes a group is cut out of two aligned vectors, so that a thread's elements,
+  // and with them the order of every sum, do not depend on where the row lies.
+  const int shift = (int)((uintptr_t)logits & 15);  // in bytes
+  L* slice = reinterpret_cast<L*>(slice_raw);
+  const int vectors = (n + W - 1) / W;
   for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = total[b] = 0;
-  if (tid == 0) sh_count = 0;
-  float top = -INFINITY;
-  const auto put = [&](int i, L x) {
-    float t = to_f32<L>(x) / div + 0.f;
-    t = isnan(t) ? -INFINITY : t;
-    t_s[i] = t;
-    top = fmaxf(top, t);
-  };
+  float greatest = -INFINITY;  // of this thread's
   {
-    constexpr int W = 16 / sizeof(L);  // elements of a 16-byte load
-    const int head = min(n, (int)((16 - ((uintptr_t)logits & 15)) & 15) / (int)sizeof(L));
-    const int vectors = (n - head) / W, tail = head + vectors * W;
-    if (tid < head) put(tid, logits[tid]);
-    const uint4* from = reinterpret_cast<const uint4*>(logits + head);
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(logits) - shift);
+    const int ahead = shift ? W : 0;
+#pragma unroll 4
     for (int v = tid; v < vectors; v += kSliceThreads) {
-      const uint4 x = __ldcs(from + v);
-      const L* e = reinterpret_cast<const L*>(&x);
+      uint4 x;
+      L* e = reinterpret_cast<L*>(&x);
+      if ((shift == 0 || v > 0) && (v + 1) * W + ahead <= n) {
+        x = from[v];
+        if (shift) {
+          const uint4 y = from[v + 1];
+          const uint32_t bits = (shift & 3) * 8;
+          uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          if (shift & 8) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) put(head + v * W + j, e[j]);
+            for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+          }
+          if (shift & 4) {
+#pragma unroll
+            for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+          }
+          x = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                         __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          e[j] = v * W + j < n ? logits[v * W + j] : from_f32<L>(-INFINITY);
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        e[j] = not_nan(e[j]);
+        greatest = fmaxf(greatest, to_f32<L>(e[j]));
+      }
+      slice_raw[v] = x;
     }
-    if (tail + tid < n) put(tail + tid, logits[tail + tid]);
   }
-  top = (float)over_cluster(block_max(top), 0., most).x;
+  float top = (float)over_cluster(block_max(greatest), 0., most).x;
   if (top == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -352,373 +384,399 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
     return;
   }
   if (top == INFINITY) {  // infinite logits share all the probability
-    for (int i = tid; i < n; i += kSliceThreads) t_s[i] = t_s[i] == INFINITY ? 0.f : -INFINITY;
+    for (int i = tid; i < n; i += kSliceThreads)
+      slice[i] = from_f32<L>(to_f32<L>(slice[i]) == INFINITY ? 0.f : -INFINITY);
+    greatest = greatest == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
     __syncthreads();
   }
+  // f(value, index in the slice) for every finite logit; a thread's come in rising order
+  const auto each = [&](auto f) {
+    for (int v = tid; v < vectors; v += kSliceThreads) {
+      const uint4 x = slice_raw[v];
+      const L* e = reinterpret_cast<const L*>(&x);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float l = to_f32<L>(e[j]);
+        if (l > -INFINITY) f(l, v * W + j);
+      }
+    }
+  };
+  const float per_unit = fminf(kLog2e / div, FLT_MAX);
+  const auto weight = [&](float l) { return exp2_approx((l - top) * per_unit); };
+  const float top_t = top / div;
 
-  // ---- sum of the weights; histogram of the steps below the greatest
+  // ---- sum of the weights, and the threads' greatest in steps below the greatest
   const bool limited = hot && (k < V || p < 1.f);
-  const auto weight = [&](float t) { return __expf(t - top); };
-  // Bins of the values up to hi: at first by value, 1/32 each and the last one open; when a cut is
-  // narrowed down, by ordered key between the least and the greatest key in reach, which puts
-  // those two in different bins however near they are.
+  // Bins of the logits up to hi: at first by value, the last one open; when a cut is narrowed
+  // down, by ordered key between the least and the greatest key in reach, which puts those two
+  // in different bins however near they are.
+  const float bins_per_logit = fminf(kBinsPerUnit / div, FLT_MAX);
   float hi = top;
   uint64_t key_scale = 0;  // bins per key, times 2^32
-  const auto bin_of = [&](float t) {
-    if (key_scale) return (int)((uint64_t)(order_key(hi) - order_key(t)) * key_scale >> 32);
-    return min((int)((hi - t) * kBinsPerUnit), kBins - 1);
+  const auto bin_of = [&](float l) {
+    if (key_scale) return (int)((uint64_t)(order_key(hi) - order_key(l)) * key_scale >> 32);
+    return min((int)((hi - l) * bins_per_logit), kBins - 1);
   };
-  // log-weights that the elements of bin b lie between
+  // the logits of bin b are at most this, and those of the bins after it below it
   const auto upper_edge = [&](int b) {
-    if (!key_scale) return hi - top - b / kBinsPerUnit;
+    if (!key_scale) return hi - b / bins_per_logit;
     const uint64_t off = (((uint64_t)b << 32) + key_scale - 1) / key_scale;
-    return key_value((uint32_t)max((int64_t)order_key(hi) - (int64_t)off, (int64_t)0x00800000)) - top;
+    return key_value((uint32_t)max((int64_t)order_key(hi) - (int64_t)off, (int64_t)0x00800000));
   };
-  {
-    float z = 0.f;
-    int finite = 0;
-    for (int i = tid; i < n; i += kSliceThreads) {
-      const float t = t_s[i];
-      z += weight(t);
-      if (limited && t > -INFINITY) {
-        atomicAdd(&hist[bin_of(t)], 1u);
-        ++finite;
-      }
+  // this block's histogram added to block 0's
+  const auto pool_hist = [&] {
+    uint32_t* all = cluster.map_shared_rank(total, 0);
+    for (int b = tid; b < kBins; b += kSliceThreads)
+      if (hist[b]) atomicAdd(all + b, hist[b]);
+  };
+
+  float z = 0.f;
+  int finite = 0;
+  for (int v = tid; v < vectors; v += kSliceThreads) {
+    const uint4 x = slice_raw[v];
+    const L* e = reinterpret_cast<const L*>(&x);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float l = to_f32<L>(e[j]);
+      z += weight(l);
+      finite += l > -INFINITY;
     }
-    dpart[0] = 0.;
-    __syncthreads();
-    const double zs = block_sum(z), fs = block_sum(finite);
-    const auto pool_hist = [&] {
-      uint32_t* all = cluster.map_shared_rank(total, 0);
-      for (int b = tid; b < kBins; b += kSliceThreads)
-        if (hist[b]) atomicAdd(all + b, hist[b]);
-    };
-    if (limited) pool_hist();
-    const double2 both = over_cluster(zs, fs, add);
-    const double Z = both.x;
-    const int usable = (int)both.y;
-    const float log_z = logf((float)Z);
-    const auto answer = [&](int index, float t) {
-      a.tokens[row] = index;
-      if (a.logprobs) a.logprobs[row] = (t - top) - log_z;
-    };
+  }
+  if (limited && greatest > -INFINITY) atomicAdd(&hist[bin_of(greatest)], 1u);
+  const double zs = block_sum(z), fs = block_sum(finite);
+  if (limited) pool_hist();
+  const double2 both = over_cluster(zs, fs, add);
+  const double Z = both.x;
+  const int usable = (int)both.y;
+  const float log_z = logf((float)Z);
+  const auto answer = [&](int index, float l) {
+    a.tokens[row] = index;
+    if (a.logprobs) a.logprobs[row] = (l == top ? 0.f : l / div - top_t) - log_z;
+  };
+  const auto heavy_enough = [&](float l) {
+    const float t = l / div;
+    return t == top_t || expf(t - top_t) >= least_weight;
+  };
+  const auto key_of = [&](float l, float e) {  // t - log(noise), a NaN last
+    const float s = l / div - logf(e);
+    return isnan(s) ? -INFINITY : s;
+  };
 
-    // t - log(noise) of the slice's element i against the best so far, the logarithm in full only
-    // where its approximation comes within 1e-3
-    const auto consider = [&](Best& best, int i, float t, float e) {
-      if (!(t - __logf(e) < best.value - 1e-3f)) {
-        float s = t - logf(e);
-        if (isnan(s)) s = -INFINITY;
-        best = better(best, {s, first + i});
+  if (limited) {
+    uint32_t* all = cluster.map_shared_rank(total, 0);
+    const auto fetch = [&] {
+      for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = all[b];
+      __syncthreads();
+    };
+    // Bins that hold a cut: by count the one where `want` is reached, by mass those where it may
+    // be, given `above` over bin 0.  x, y: first and last of them; z, w: counts up to the first
+    // (exclusive) and the last (inclusive).  `reached`: the lower bound got there at all.
+    bool reached;
+    const auto find_bins = [&](bool by_mass, double want, double above, bool open_end) {
+      if (tid == 0) sh_bin[0] = sh_bin[1] = kBins;
+      const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+      double lo0 = c0, lo1 = c1, up0 = c0, up1 = c1;
+      if (by_mass) {
+        const auto edge = [&](int b) { return (double)weight(upper_edge(b)); };
+        lo0 *= edge(2 * tid + 1) * (1. - 1e-4);
+        lo1 *= open_end && 2 * tid + 1 == kBins - 1 ? 0. : edge(2 * tid + 2) * (1. - 1e-4);
+        up0 *= edge(2 * tid) * (1. + 1e-4);
+        up1 *= edge(2 * tid + 1) * (1. + 1e-4);
       }
+      double all_lo, all_up;
+      __syncthreads();
+      const double through_lo = block_scan_inclusive(lo0 + lo1, dpart, all_lo) + above;
+      const double through_up = block_scan_inclusive(up0 + up1, dpart, all_up) + above;
+      if (c0 && through_up - up1 >= want) atomicMin(&sh_bin[0], 2 * tid);
+      if (c1 && through_up >= want) atomicMin(&sh_bin[0], 2 * tid + 1);
+      if (c0 && through_lo - lo1 >= want) atomicMin(&sh_bin[1], 2 * tid);
+      if (c1 && through_lo >= want) atomicMin(&sh_bin[1], 2 * tid + 1);
+      // not reached: the last bin that holds anything
+      const int last = (int)block_max((float)(c1 ? 2 * tid + 1 : c0 ? 2 * tid : -1));
+      const int b1 = min(sh_bin[0], last), b2 = min(sh_bin[1], last);
+      reached = sh_bin[1] < kBins;
+      int sum;
+      const int through = block_scan_inclusive((int)(c0 + c1), ipart, sum);
+      if (2 * tid == (b1 & ~1)) sh_bin[0] = through - (int)(c0 + c1) + (b1 & 1 ? (int)c0 : 0);
+      if (2 * tid == (b2 & ~1)) sh_bin[1] = through - (b2 & 1 ? 0 : (int)c1);
+      __syncthreads();
+      const int4 r = make_int4(b1, b2, sh_bin[0], sh_bin[1]);
+      __syncthreads();
+      return r;
     };
-    const auto heavy_enough = [&](float t) {
-      return t == top || expf(t - top) >= least_weight;
+    // Gathers the logits from `least` to hi with bins b1 .. b2 in block 0, if at most
+    // kCandidates, and ranks them in its own_l, own_i; cluster barriers.  Returns their number.
+    const auto gather = [&](float least, int b1, int b2) {
+      if (tid == 0) sh_count = 0;
+      __syncthreads();
+      const float edge = key_scale ? least : fmaxf(least, upper_edge(b2 + 1) - 1.f / bins_per_logit);
+      each([&](float l, int i) {
+        // a compare first: the bins' exact test for few (the edge is one step too low)
+        if (l < edge && b2 < kBins - 1) return;
+        if (l < least || l > hi) return;
+        const int b = bin_of(l);
+        if (b < b1 || b > b2) return;
+        const int at = atomicAdd(&sh_count, 1);
+        if (at < kCandidates) own_l[at] = l, own_i[at] = first + i;
+      });
+      __syncthreads();
+      const int mine = sh_count;
+      double(*box)[2] = sums.v[turn & 1];
+      const int m = (int)over_cluster(mine, 0., add).x;
+      if (m > kCandidates) return m;
+      int before = 0;
+      for (int r = 0; r < rank; ++r) before += (int)box[r][0];
+      float* to_l = cluster.map_shared_rank(cand_l, 0);
+      int* to_i = cluster.map_shared_rank(cand_i, 0);
+      for (int j = tid; j < mine; j += kSliceThreads) {
+        to_l[before + j] = own_l[j];
+        to_i[before + j] = own_i[j];
+      }
+      cluster.sync();
+      if (rank == 0) {
+        if (tid < m) {
+          const float l = cand_l[tid];
+          const int i = cand_i[tid];
+          int r = 0;
+          for (int j = 0; j < m; ++j) r += cand_l[j] > l || (cand_l[j] == l && cand_i[j] < i);
+          own_l[r] = l;
+          own_i[r] = i;
+        }
+        __syncthreads();
+      }
+      return m;
+    };
+    // All limits on a ranked list that holds every token kept; block 0 alone.
+    const bool by_count = k < usable;
+    const auto finish = [&](int m) {
+      const bool in = tid < m && (!by_count || tid < k);
+      const float l = in ? own_l[tid] : -INFINITY;
+      const double w = in ? (double)weight(l) : 0.;
+      double kept_mass;
+      const double before = block_scan_inclusive(w, dpart, kept_mass) - w;
+      const double target = p < 1.f ? p * (by_count ? kept_mass : Z) : INFINITY;
+      Best best = {-INFINITY, INT32_MAX};
+      if (in && (tid == 0 || before < target) && heavy_enough(l))
+        best = {key_of(l, a.noise[row * a.noise_stride + own_i[tid]]), own_i[tid]};
+      const Best won = block_best(best, part);
+      if (in && best.index == won.index) answer(won.index, l);
     };
 
-    if (limited) {
-      uint32_t* all = cluster.map_shared_rank(total, 0);
-      // exclusive prefix of counts over the bins, two bins a thread
-      const auto fetch = [&] {
-        for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = all[b];
-        __syncthreads();
-      };
-      fetch();
-      // Bins that hold a cut: by count the one where `want` is reached, by mass those where
-      // `target` may be, given `above` (count or mass) over bin 0.  In sh_bin, last bin inclusive;
-      // returns the counts up to the first of them (exclusive) and the last (inclusive).
-      const auto find_bins = [&](bool by_mass, double want, double above, bool open_end) {
-        if (tid == 0) sh_bin[0] = sh_bin[1] = kBins;
-        const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-        double lo0 = c0, lo1 = c1, up0 = c0, up1 = c1;
-        if (by_mass) {
-          const auto edge = [&](int b) { return (double)__expf(upper_edge(b)); };
-          lo0 *= edge(2 * tid + 1) * (1. - 1e-4);
-          lo1 *= open_end && 2 * tid + 1 == kBins - 1 ? 0. : edge(2 * tid + 2) * (1. - 1e-4);
-          up0 *= edge(2 * tid) * (1. + 1e-4);
-          up1 *= edge(2 * tid + 1) * (1. + 1e-4);
-        }
-        double all_lo, all_up;
-        __syncthreads();
-        const double through_lo = block_scan_inclusive(lo0 + lo1, dpart, all_lo) + above;
-        const double through_up = block_scan_inclusive(up0 + up1, dpart, all_up) + above;
-        if (c0 && through_up - up1 >= want) atomicMin(&sh_bin[0], 2 * tid);
-        if (c1 && through_up >= want) atomicMin(&sh_bin[0], 2 * tid + 1);
-        if (c0 && through_lo - lo1 >= want) atomicMin(&sh_bin[1], 2 * tid);
-        if (c1 && through_lo >= want) atomicMin(&sh_bin[1], 2 * tid + 1);
-        __syncthreads();
-        // not reached: the last bins that hold anything
-        int last = c1 ? 2 * tid + 1 : c0 ? 2 * tid : -1;
-        last = (int)block_max((float)last);
-        const int b1 = min(sh_bin[0], last), b2 = min(sh_bin[1], last);
-        int sum;
-        const int through = block_scan_inclusive((int)(c0 + c1), ipart, sum);
-        __syncthreads();
-        if (2 * tid == (b1 & ~1)) sh_bin[0] = through - (int)(c0 + c1) + (b1 & 1 ? (int)c0 : 0);
-        if (2 * tid == (b2 & ~1)) sh_bin[1] = through - (b2 & 1 ? 0 : (int)c1);
-        __syncthreads();
-        const int4 r = make_int4(b1, b2, sh_bin[0], sh_bin[1]);
-        __syncthreads();
-        return r;
-      };
-      // Gathers the elements from `least` to hi with bins b1 .. b2, at most kCandidates, in block
-      // 0 and ranks them there; a cluster barrier.
-      const auto gather = [&](float least, int b1, int b2) {
-        int* count = cluster.map_shared_rank(&sh_count, 0);
-        float* ct = cluster.map_shared_rank(cand_t, 0);
-        int* ci = cluster.map_shared_rank(cand_i, 0);
-        for (int i = tid; i < n; i += kSliceThreads) {
-          const float t = t_s[i];
-          if (!(t > -INFINITY) || t < least || t > hi) continue;
-          const int b = bin_of(t);
-          if (b < b1 || b > b2) continue;
-          const int at = atomicAdd(count, 1);
-          if (at < kCandidates) {
-            ct[at] = t;
-            ci[at] = first + i;
-          }
-        }
-        cluster.sync();
-        if (rank == 0) {
-          const int m = min(sh_count, kCandidates);
-          if (tid < m) {
-            const float t = cand_t[tid];
-            const int i = cand_i[tid];
-            int r = 0;
-            for (int j = 0; j < m; ++j)
-              r += cand_t[j] > t || (cand_t[j] == t && cand_i[j] < i);
-            rank_t[r] = t;
-            rank_i[r] = i;
-          }
-          __syncthreads();
-          return m;
-        }
-        return 0;
-      };
-
-      const bool by_count = k < usable;
-      int4 bins = by_count ? find_bins(false, k, 0., true) : find_bins(true, p * Z, 0., true);
-      if ((by_count || p < 1.f) && bins.w <= kCandidates) {
-        // ---- few enough: all limits on the ranked list
-        const int m = gather(-INFINITY, 0, bins.y);
-        if (rank != 0) return;
-        const bool in = tid < m && (!by_count || tid < k);
-        const float t = in ? rank_t[tid] : -INFINITY;
-        const double w = in ? (double)weight(t) : 0.;
-        double kept_mass;
-        const double before = block_scan_inclusive(w, dpart, kept_mass) - w;
-        const double target = p < 1.f ? p * (by_count ? kept_mass : Z) : INFINITY;
-        Best best = {-INFINITY, INT32_MAX};
-        if (in && (tid == 0 || before < target) && heavy_enough(t)) {
-          float s = t - logf(a.noise[row * a.noise_stride + rank_i[tid]]);
-          if (isnan(s)) s = -INFINITY;
-          best = {s, rank_i[tid]};
-          cand_t[tid] = t;
-        }
-        const Best won = block_best(best, part);
-        if (in && best.index == won.index) answer(won.index, t);
+    fetch();
+    int4 bins = find_bins(!by_count, by_count ? (double)k : (double)p * Z, 0., true);
+    if ((by_count || p < 1.f) && reached && bins.w <= kCandidates) {
+      const int m = gather(-INFINITY, 0, bins.y);
+      if (m <= kCandidates) {
+        if (rank == 0) finish(m);
         return;
       }
+    }
 
-      // ---- cuts by narrowing
-      for (int limit = 0; limit < 2; ++limit) {  // top_k, then top_p
-        const bool by_mass = limit == 1;
-        if (by_mass ? !(p < 1.f) : !by_count) continue;
-        double want = k, above = 0., mass = 0.;
-        if (by_mass) {
-          mass = Z;
-          if (by_count) {  // what top_k left
-            float z = 0.f;
-            for (int i = tid; i < n; i += kSliceThreads) z += weight(t_s[i]);
-            mass = over_cluster(block_sum(z), 0., add).x;
-          }
-          want = p * mass;
+    // ---- cuts by narrowing
+    cluster.sync();  // every block has read the pooled histogram, which is cleared next
+    for (int limit = 0; limit < 2; ++limit) {  // top_k, then top_p
+      const bool by_mass = limit == 1;
+      if (by_mass ? !(p < 1.f) : !by_count) continue;
+      double want = k, above = 0.;
+      if (by_mass) {
+        double mass = Z;
+        if (by_count) {  // what top_k left
+          float left = 0.f;
+          each([&](float l, int) { left += weight(l); });
+          mass = over_cluster(block_sum(left), 0., add).x;
         }
-        bool open_end = true;
-        int above_count = 0;
-        for (int level = 0;; ++level) {
-          if (level > 0 || (by_mass && by_count)) {  // histogram of the elements in reach
-            if (level == 0) hi = top, key_scale = 0;
-            for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = total[b] = 0;
-            cluster.sync();
-            for (int i = tid; i < n; i += kSliceThreads) {
-              const float t = t_s[i];
-              if (!(t > -INFINITY) || t > hi) continue;
-              if (level > 0 && t < sh_cut) continue;
-              atomicAdd(&hist[bin_of(t)], 1u);
-            }
-            __syncthreads();
-            for (int b = tid; b < kBins; b += kSliceThreads)
-              if (hist[b]) atomicAdd(all + b, hist[b]);
-            cluster.sync();
-            fetch();
-          }
-          bins = find_bins(by_mass, by_mass ? want : want - above_count, by_mass ? above : 0.,
-                           open_end);
-          if (by_mass && level > 0 && bins.x == 0 && bins.y == bin_of(sh_cut)) {
-            // the bounds leave every bin (coarse ones, or few values many times): the exact mass
-            // of the upper half of the bins decides between the halves, and neither is empty,
-            // since hi is in the first bin and the least value in the last
-            const int half = bins.y / 2;
-            float z = 0.f;
-            int count = 0;
-            for (int i = tid; i < n; i += kSliceThreads) {
-              const float t = t_s[i];
-              if (!(t > -INFINITY) || t < sh_cut || t > hi || bin_of(t) > half) continue;
-              z += weight(t);
-              ++count;
-            }
-            const double2 upper = over_cluster(block_sum(z), block_sum(count), add);
-            if (above + upper.x >= want) bins.y = half, bins.w = (int)upper.y;
-            else bins.x = half + 1, bins.z = (int)upper.y;
-          }
-          // mass (or count) above the bins; range of the values in them
-          float z = 0.f, low = INFINITY, high = -INFINITY;
-          for (int i = tid; i < n; i += kSliceThreads) {
-            const float t = t_s[i];
-            if (!(t > -INFINITY) || t > hi) continue;
-            if (level > 0 && t < sh_cut) continue;
-            const int b = bin_of(t);
-            if (b < bins.x) z += weight(t);
-            else if (b <= bins.y) low = fminf(low, t), high = fmaxf(high, t);
-          }
-          above += over_cluster(block_sum(z), 0., add).x;
-          const double2 range = over_cluster(block_max(-low), block_max(high), most);
-          low = -(float)range.x;
-          high = (float)range.y;
-          const int members = bins.w - bins.z;
-          above_count += bins.z;
-          __syncthreads();
-          if (low == high || level >= 64) {  // ties: as many as the limit still takes
-            if (tid == 0) {
-              const double w = weight(low);
-              const double takes = !by_mass ? want - above_count
-                                   : w > 0. ? ceil((want - above) / w) : 1.;
-              sh_cut = low;
-              sh_ties = (int)fmin(fmax(takes, above_count ? 0. : 1.), (double)members);
-            }
-            __syncthreads();
-            break;
-          }
-          if (members <= kCandidates) {
-            const int m = gather(level > 0 ? sh_cut : -INFINITY, bins.x, bins.y);
-            if (rank == 0) {
-              const float t = tid < m ? rank_t[tid] : -INFINITY;
-              const double w = tid < m ? (double)weight(t) : 0.;
-              double unused;
-              const double before = above + block_scan_inclusive(w, dpart, unused) - w;
-              const bool in = tid < m && (by_mass ? before < want || (above_count == 0 && tid == 0)
-                                                  : above_count + tid < want);
-              const int kept = max((int)block_sum(in ? 1. : 0.), 1);
-              const float cut = rank_t[kept - 1];
-              const int ties = (int)block_sum(tid < kept && t == cut ? 1. : 0.);
-              if (tid < ranks) {
-                *cluster.map_shared_rank(&sh_cut, tid) = cut;
-                *cluster.map_shared_rank(&sh_ties, tid) = ties;
-              }
-              if (tid == 0) sh_count = 0;
-            }
-            cluster.sync();
-            break;
-          }
-          // narrower: the values between low and high
-          if (tid == 0) sh_cut = low;
-          hi = high;
-          key_scale = ((uint64_t)kBins << 32) / ((uint64_t)order_key(high) - order_key(low) + 1);
-          open_end = false;
-          __syncthreads();
+        want = p * mass;
+      }
+      hi = top;
+      key_scale = 0;
+      float least = -INFINITY;
+      int above_count = 0;
+      for (int level = 0;; ++level) {
+        // histogram of the logits from `least` to hi
+        for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = total[b] = 0;
+        cluster.sync();
+        each([&](float l, int) {
+          if (l >= least && l <= hi) atomicAdd(&hist[bin_of(l)], 1u);
+        });
+        __syncthreads();
+        pool_hist();
+        cluster.sync();
+        fetch();
+        bins = find_bins(by_mass, by_mass ? want : want - above_count, by_mass ? above : 0.,
+                         level == 0);
+        if (by_mass && level > 0 && bins.x == 0 && bins.y == bin_of(least)) {
+          // the bounds leave every bin (coarse ones, or few values many times): the exact mass
+          // of the upper half of the bins decides between the halves, and neither is empty,
+          // since hi is in the first bin and the least value in the last
+          const int half = bins.y / 2;
+          float up = 0.f;
+          int count = 0;
+          each([&](float l, int) {
+            if (l < least || l > hi || bin_of(l) > half) return;
+            up += weight(l);
+            ++count;
+          });
+          const double2 upper = over_cluster(block_sum(up), block_sum(count), add);
+          if (above + upper.x >= want) bins.y = half, bins.w = (int)upper.y;
+          else bins.x = half + 1, bins.z = (int)upper.y;
         }
-        // strike out what is below the cut, and the ties past the last one kept
-        const float cut = sh_cut;
-        const int ties = sh_ties;
-        int mine = 0;
-        for (int i = tid; i < n; i += kSliceThreads) mine += t_s[i] == cut;
-        mine = (int)block_sum(mine);
-        double(*box)[2] = sums.v[turn & 1];
-        over_cluster(mine, 0., add);
-        int before = 0;
-        for (int r = 0; r < rank; ++r) before += (int)box[r][0];
-        const int keeps = min(max(ties - before, 0), mine);
-        int seen = 0;
-        for (int i0 = 0; i0 < n; i0 += kSliceThreads) {
-          const int i = i0 + tid;
-          const float t = i < n ? t_s[i] : INFINITY;
-          if (keeps == 0 || keeps == mine) {
-            if (t < cut || (t == cut && keeps == 0)) t_s[i] = -INFINITY;
-            continue;
+        const int members = bins.w - bins.z;
+        above_count += bins.z;
+        // mass above the bins; range of the values in them
+        float up = 0.f, low = INFINITY, high = -INFINITY;
+        each([&](float l, int) {
+          if (l < least || l > hi) return;
+          const int b = bin_of(l);
+          if (b < bins.x) up += weight(l);
+          else if (b <= bins.y) low = fminf(low, l), high = fmaxf(high, l);
+        });
+        above += over_cluster(block_sum(up), 0., add).x;
+        const double2 range = over_cluster(block_max(-low), block_max(high), most);
+        low = -(float)range.x;
+        high = (float)range.y;
+        if (low == high || level >= 64) {  // ties: as many as the limit still takes
+          if (tid == 0) {
+            const double w = weight(low);
+            const double takes = !by_mass ? want - above_count
+                                 : w > 0. ? ceil((want - above) / w) : 1.;
+            sh_cut = low;
+            sh_ties = (int)fmin(fmax(takes, above_count ? 0. : 1.), (double)members);
           }
+          __syncthreads();
+          break;
+        }
+        if (members <= kCandidates) {
+          const int m = gather(least, bins.x, bins.y);
+          if (rank == 0) {
+            const float l = tid < m ? own_l[tid] : -INFINITY;
+            const double w = tid < m ? (double)weight(l) : 0.;
+            double unused;
+            const double before = above + block_scan_inclusive(w, dpart, unused) - w;
+            const bool in = tid < m && (by_mass ? before < want || (above_count == 0 && tid == 0)
+                                                : above_count + tid < want);
+            const int kept = max((int)block_sum(in ? 1. : 0.), 1);
+            const float cut = own_l[kept - 1];
+            const int ties = (int)block_sum(tid < kept && l == cut ? 1. : 0.);
+            if (tid < ranks) {
+              *cluster.map_shared_rank(&sh_cut, tid) = cut;
+              *cluster.map_shared_rank(&sh_ties, tid) = ties;
+            }
+          }
+          cluster.sync();
+          break;
+        }
+        // narrower: the values between low and high
+        least = low;
+        hi = high;
+        key_scale = ((uint64_t)kBins << 32) / ((uint64_t)order_key(high) - order_key(low) + 1);
+      }
+      // strike out what is below the cut, and the ties past the last one kept
+      const float cut = sh_cut;
+      const int ties = sh_ties;
+      int mine = 0;
+      each([&](float l, int) { mine += l == cut; });
+      mine = (int)block_sum(mine);
+      double(*box)[2] = sums.v[turn & 1];
+      over_cluster(mine, 0., add);
+      int before = 0;
+      for (int r = 0; r < rank; ++r) before += (int)box[r][0];
+      const int keeps = min(max(ties - before, 0), mine);
+      int seen = 0;
+      for (int i0 = 0; i0 < n; i0 += kSliceThreads) {
+        const int i = i0 + tid;
+        const float l = i < n ? to_f32<L>(slice[i]) : INFINITY;
+        bool out = l < cut;
+        if (keeps == 0) {
+          out |= l == cut;
+        } else if (keeps < mine) {
           int count;
-          const int through = seen + block_scan_inclusive((int)(t == cut), ipart, count);
-          if (t < cut || (t == cut && through > keeps)) t_s[i] = -INFINITY;
+          const int through = seen + block_scan_inclusive((int)(l == cut), ipart, count);
+          out |= l == cut && through > keeps;
           seen += count;
         }
-        __syncthreads();
+        if (out) slice[i] = from_f32<L>(-INFINITY);
       }
+      __syncthreads();
     }
+  }
 
-    // ---- the best of what is left
-    Best best = {-INFINITY, INT32_MAX};
-    if (!hot) {
-      for (int i = tid; i < n; i += kSliceThreads) best = better(best, {t_s[i], first + i});
-    } else if (least_weight > 0.f) {
-      const float sure = top + logf(least_weight);
-      for (int i = tid; i < n; i += kSliceThreads) {
-        const float t = t_s[i];
-        if (!(t > -INFINITY) || t < sure - 1e-3f || !heavy_enough(t)) continue;
-        consider(best, i, t, noise[i]);
-      }
+  // ---- the best of what is left
+  Best best = {-INFINITY, INT32_MAX};
+  float best_l = 0.f;
+  if (!hot) {
+    each([&](float l, int i) {
+      if (l == top && first + i < best.index) best = {l, first + i}, best_l = l;
+    });
+  } else {
+    // The logarithm in full only where its approximation comes within 1e-3 of the best so far
+    // (t within 2^-22 of |t| by the reciprocal's rounding, below that for |t| up to 2000).
+    const float inv = 1.f / div;
+    const float sure = least_weight > 0.f ? (top_t + logf(least_weight)) - 1e-3f : -INFINITY;
+    const auto consider = [&](float l, int i, float e) {
+      const float t = l * inv;
+      if (t - __logf(e) < best.value - 1e-3f - fabsf(t) * 5e-7f) return;
+      const Best b = {key_of(l, e), first + i};
+      if (b.value > best.value || (b.value == best.value && b.index < best.index)) best = b, best_l = l;
+    };
+    if (least_weight > 0.f) {
+      each([&](float l, int i) {
+        if (l * inv + fabsf(l * inv) * 5e-7f < sure || !heavy_enough(l)) return;
+        consider(l, i, noise[i]);
+      });
     } else {
-      for (int i0 = tid; i0 < n; i0 += 4 * kSliceThreads) {
-        float e[4], t[4];
+      for (int i0 = tid; i0 < n; i0 += 8 * kSliceThreads) {
+        float e[8], l[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
           const int i = i0 + j * kSliceThreads;
-          t[j] = i < n ? t_s[i] : -INFINITY;
-          e[j] = t[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
+          l[j] = i < n ? to_f32<L>(slice[i]) : -INFINITY;
+          e[j] = l[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (t[j] > -INFINITY) consider(best, i0 + j * kSliceThreads, t[j], e[j]);
+        for (int j = 0; j < 8; ++j)
+          if (l[j] > -INFINITY) consider(l[j], i0 + j * kSliceThreads, e[j]);
       }
     }
-    best = block_best(best, part);
-    if (tid == 0) {
-      cluster.map_shared_rank(cluster_best, 0)[rank] = best;
-      // the value of the block's best, for the logprob
-      cluster.map_shared_rank(cluster_t, 0)[rank] = best.index < V ? t_s[best.index - first] : 0.f;
-    }
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-      int who = 0;
-      for (int r = 1; r < ranks; ++r)
-        if (cluster_best[r].value > cluster_best[who].value ||
-            (cluster_best[r].value == cluster_best[who].value &&
-             cluster_best[r].index < cluster_best[who].index))
-          who = r;
-      answer(cluster_best[who].index, cluster_t[who]);
-    }
+  }
+  const Best own = best;
+  best = block_best(best, part);
+  if (own.index == best.index && best.index < V) {
+    cluster.map_shared_rank(cluster_best, 0)[rank] = best;
+    cluster.map_shared_rank(cluster_l, 0)[rank] = best_l;
+  } else if (tid == 0 && best.index >= V) {  // nothing of this slice is left
+    cluster.map_shared_rank(cluster_best, 0)[rank] = best;
+  }
+  cluster.sync();
+  if (rank == 0 && tid == 0) {
+    int who = 0;
+    for (int r = 1; r < ranks; ++r)
+      if (cluster_best[r].value > cluster_best[who].value ||
+          (cluster_best[r].value == cluster_best[who].value &&
+           cluster_best[r].index < cluster_best[who].index))
+        who = r;
+    answer(cluster_best[who].index, cluster_l[who]);
   }
 }
 
 template <typename L>
 static int launch_sample(const SampleArgs& a, int64_t rows, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.vocab > 8 * kMaxSlice) {  // does not fit the cluster's shared memory
+  if ((int64_t)a.vocab * (int)sizeof(L) > 8 * kMaxSliceBytes) {  // more than a cluster holds
     sample_kernel<L><<<(unsigned)rows, kSampleThreads, 0, s>>>(a);
     return serve_launched("tr_sample");
   }
-  // blocks per row: slices of 16384 where the rows fill the GPU, 8 blocks where they do not
+  // blocks per row: as many as hold it in 64 KB each, more where the rows leave SMs idle
   int blocks = 1;
-  while (blocks < 8 && (a.vocab > blocks * 16384 ||
+  while (blocks < 8 && (a.vocab * (int)sizeof(L) > blocks * kSliceBytes ||
                         (a.vocab > blocks * 2048 && rows * blocks * 2 <= serve_sms())))
     blocks *= 2;
   const int slice = (a.vocab + blocks - 1) / blocks;
-  const size_t smem = (size_t)slice * sizeof(float);
+  const size_t smem = ((size_t)slice * sizeof(L) + 15) / 16 * 16;
   auto kernel = sample_cluster_kernel<L>;
-  if (smem > 30 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float));
+  if (smem > 24 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSliceBytes + 64);
     if (e != cudaSuccess) {
       set_error("tr_sample: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
       return TR_ERR_CUDA;
