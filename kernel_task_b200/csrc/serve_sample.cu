@@ -239,15 +239,20 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 // steps below the greatest (1/32 of t each), summed over the cluster: these are some of the
 // tokens, so where they alone reach top_k, or top_p of the mass, all tokens kept lie in the steps
 // down to there.  They are gathered, ranked, and all limits applied to the ranked list; noise is
-// read for them alone.  Where they do not reach, or are over kCandidates, all logits are
-// counted, and each limit's cut is narrowed down by further histograms over the steps that can
-// hold it (for a mass: between the bounds that the steps' edges give, with the exact mass above
-// them) until few enough tokens or a single value is left; what is below the cut is struck out.
+// read for them alone.
+//
+// Where that does not do, one limit needs no cut: the token drawn from all, if the limit keeps
+// it (its rank, or the mass above it, is one pass), is the token drawn from the kept; if not, the
+// kept are among those ranked above it, and one of these is drawn.  The first draw is kept with
+// the kept tokens' probability, and every other draw halves what is left or so.  After
+// kDraws, and for top_k where the mass of what it keeps is asked for, the cut is searched by
+// halving the ordered keys until few enough tokens for a ranked list lie between.
 // All sums run in an order fixed by the row alone.
 constexpr int kSliceThreads = 512;
 constexpr int kBins = 1024;
 constexpr float kBinsPerUnit = 32.f;
 constexpr int kCandidates = 512;
+constexpr int kDraws = 12;
 constexpr int kSliceBytes = 65536;     // of a block where the rows fill the GPU: three blocks an SM
 constexpr int kMaxSliceBytes = 200000;
 
@@ -272,9 +277,9 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   __shared__ int own_i[kCandidates], cand_i[kCandidates];
   __shared__ Best part[32], cluster_best[8];
   __shared__ double dpart[32];
-  __shared__ float fpart[32], cluster_l[8];
+  __shared__ float fpart[32];
   __shared__ int ipart[32];
-  __shared__ int sh_count, sh_bin[2], sh_ties;
+  __shared__ int sh_count, sh_bin, sh_ties;
   __shared__ float sh_cut;
 
   const cg::cluster_group cluster = cg::this_cluster();
@@ -408,28 +413,8 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
 
   // ---- sum of the weights, and the threads' greatest in steps below the greatest
   const bool limited = hot && (k < V || p < 1.f);
-  // Bins of the logits up to hi: at first by value, the last one open; when a cut is narrowed
-  // down, by ordered key between the least and the greatest key in reach, which puts those two
-  // in different bins however near they are.
   const float bins_per_logit = fminf(kBinsPerUnit / div, FLT_MAX);
-  float hi = top;
-  uint64_t key_scale = 0;  // bins per key, times 2^32
-  const auto bin_of = [&](float l) {
-    if (key_scale) return (int)((uint64_t)(order_key(hi) - order_key(l)) * key_scale >> 32);
-    return min((int)((hi - l) * bins_per_logit), kBins - 1);
-  };
-  // the logits of bin b are at most this, and those of the bins after it below it
-  const auto upper_edge = [&](int b) {
-    if (!key_scale) return hi - b / bins_per_logit;
-    const uint64_t off = (((uint64_t)b << 32) + key_scale - 1) / key_scale;
-    return key_value((uint32_t)max((int64_t)order_key(hi) - (int64_t)off, (int64_t)0x00800000));
-  };
-  // this block's histogram added to block 0's
-  const auto pool_hist = [&] {
-    uint32_t* all = cluster.map_shared_rank(total, 0);
-    for (int b = tid; b < kBins; b += kSliceThreads)
-      if (hist[b]) atomicAdd(all + b, hist[b]);
-  };
+  const auto bin_of = [&](float l) { return min((int)((top - l) * bins_per_logit), kBins - 1); };
 
   float z = 0.f;
   int finite = 0;
@@ -445,7 +430,12 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   }
   if (limited && greatest > -INFINITY) atomicAdd(&hist[bin_of(greatest)], 1u);
   const double zs = block_sum(z), fs = block_sum(finite);
-  if (limited) pool_hist();
+  if (limited) {  // this block's histogram added to block 0's
+    uint32_t* all = cluster.map_shared_rank(total, 0);
+    __syncthreads();
+    for (int b = tid; b < kBins; b += kSliceThreads)
+      if (hist[b]) atomicAdd(all + b, hist[b]);
+  }
   const double2 both = over_cluster(zs, fs, add);
   const double Z = both.x;
   const int usable = (int)both.y;
@@ -463,60 +453,83 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
     return isnan(s) ? -INFINITY : s;
   };
 
+  // ---- the best t - log(noise) among the tokens ranked above (bound_l, bound_i); all above -inf
+  __shared__ float best_l_of[8];
+  const auto draw = [&](float bound_l, int bound_i, float& won_l) {
+    Best best = {-INFINITY, INT32_MAX};
+    float best_l = 0.f;
+    if (!hot) {
+      each([&](float l, int i) {
+        if (l == top && first + i < best.index) best = {l, first + i}, best_l = l;
+      });
+    } else {
+      // The logarithm in full only where its approximation comes within 1e-3 of the best so far;
+      // t by the reciprocal is within 2^-22 of |t|.
+      const float inv = fminf(1.f / div, FLT_MAX);
+      const float sure = least_weight > 0.f ? (top_t + logf(least_weight)) - 1e-3f : -INFINITY;
+      const auto consider = [&](float l, int i, float e) {
+        const float t = l * inv;
+        if (t - __logf(e) < best.value - 1e-3f - fabsf(t) * 5e-7f) return;
+        const Best b = {key_of(l, e), first + i};
+        if (b.value > best.value || (b.value == best.value && b.index < best.index))
+          best = b, best_l = l;
+      };
+      const auto ranked_above = [&](float l, int i) {
+        return l > bound_l || (l == bound_l && first + i < bound_i);
+      };
+      if (least_weight > 0.f) {
+        each([&](float l, int i) {
+          if (l * inv + fabsf(l * inv) * 5e-7f < sure || !ranked_above(l, i) || !heavy_enough(l))
+            return;
+          consider(l, i, noise[i]);
+        });
+      } else {
+        for (int i0 = tid; i0 < n; i0 += 8 * kSliceThreads) {
+          float e[8], l[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * kSliceThreads;
+            l[j] = i < n ? to_f32<L>(slice[i]) : -INFINITY;
+            if (!ranked_above(l[j], i)) l[j] = -INFINITY;
+            e[j] = l[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (l[j] > -INFINITY) consider(l[j], i0 + j * kSliceThreads, e[j]);
+        }
+      }
+    }
+    // over the block, then over the cluster: every block learns the winner
+    const Best own = best;
+    best = block_best(best, part);
+    if (tid == 0) fpart[0] = 0.f;
+    __syncthreads();
+    if (own.index == best.index && best.index < V) fpart[0] = best_l;
+    __syncthreads();
+    if (tid < ranks) {
+      cluster.map_shared_rank(cluster_best, tid)[rank] = best;
+      cluster.map_shared_rank(best_l_of, tid)[rank] = fpart[0];
+    }
+    cluster.sync();
+    Best won = cluster_best[0];
+    won_l = best_l_of[0];
+    for (int r = 1; r < ranks; ++r) {
+      const Best b = cluster_best[r];
+      if (b.value > won.value || (b.value == won.value && b.index < won.index))
+        won = b, won_l = best_l_of[r];
+    }
+    return won;
+  };
+
   if (limited) {
     uint32_t* all = cluster.map_shared_rank(total, 0);
-    const auto fetch = [&] {
-      for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = all[b];
-      __syncthreads();
-    };
-    // Bins that hold a cut: by count the one where `want` is reached, by mass those where it may
-    // be, given `above` over bin 0.  x, y: first and last of them; z, w: counts up to the first
-    // (exclusive) and the last (inclusive).  `reached`: the lower bound got there at all.
-    bool reached;
-    const auto find_bins = [&](bool by_mass, double want, double above, bool open_end) {
-      if (tid == 0) sh_bin[0] = sh_bin[1] = kBins;
-      const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-      double lo0 = c0, lo1 = c1, up0 = c0, up1 = c1;
-      if (by_mass) {
-        const auto edge = [&](int b) { return (double)weight(upper_edge(b)); };
-        lo0 *= edge(2 * tid + 1) * (1. - 1e-4);
-        lo1 *= open_end && 2 * tid + 1 == kBins - 1 ? 0. : edge(2 * tid + 2) * (1. - 1e-4);
-        up0 *= edge(2 * tid) * (1. + 1e-4);
-        up1 *= edge(2 * tid + 1) * (1. + 1e-4);
-      }
-      double all_lo, all_up;
-      __syncthreads();
-      const double through_lo = block_scan_inclusive(lo0 + lo1, dpart, all_lo) + above;
-      const double through_up = block_scan_inclusive(up0 + up1, dpart, all_up) + above;
-      if (c0 && through_up - up1 >= want) atomicMin(&sh_bin[0], 2 * tid);
-      if (c1 && through_up >= want) atomicMin(&sh_bin[0], 2 * tid + 1);
-      if (c0 && through_lo - lo1 >= want) atomicMin(&sh_bin[1], 2 * tid);
-      if (c1 && through_lo >= want) atomicMin(&sh_bin[1], 2 * tid + 1);
-      // not reached: the last bin that holds anything
-      const int last = (int)block_max((float)(c1 ? 2 * tid + 1 : c0 ? 2 * tid : -1));
-      const int b1 = min(sh_bin[0], last), b2 = min(sh_bin[1], last);
-      reached = sh_bin[1] < kBins;
-      int sum;
-      const int through = block_scan_inclusive((int)(c0 + c1), ipart, sum);
-      if (2 * tid == (b1 & ~1)) sh_bin[0] = through - (int)(c0 + c1) + (b1 & 1 ? (int)c0 : 0);
-      if (2 * tid == (b2 & ~1)) sh_bin[1] = through - (b2 & 1 ? 0 : (int)c1);
-      __syncthreads();
-      const int4 r = make_int4(b1, b2, sh_bin[0], sh_bin[1]);
-      __syncthreads();
-      return r;
-    };
-    // Gathers the logits from `least` to hi with bins b1 .. b2 in block 0, if at most
-    // kCandidates, and ranks them in its own_l, own_i; cluster barriers.  Returns their number.
-    const auto gather = [&](float least, int b1, int b2) {
+    // Gathers the tokens that `takes(l)` in block 0, if at most kCandidates, and ranks them in its
+    // own_l, own_i; cluster barriers.  Returns their number.
+    const auto gather = [&](auto takes) {
       if (tid == 0) sh_count = 0;
       __syncthreads();
-      const float edge = key_scale ? least : fmaxf(least, upper_edge(b2 + 1) - 1.f / bins_per_logit);
       each([&](float l, int i) {
-        // a compare first: the bins' exact test for few (the edge is one step too low)
-        if (l < edge && b2 < kBins - 1) return;
-        if (l < least || l > hi) return;
-        const int b = bin_of(l);
-        if (b < b1 || b > b2) return;
+        if (!takes(l)) return;
         const int at = atomicAdd(&sh_count, 1);
         if (at < kCandidates) own_l[at] = l, own_i[at] = first + i;
       });
@@ -547,131 +560,99 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
       }
       return m;
     };
-    // All limits on a ranked list that holds every token kept; block 0 alone.
-    const bool by_count = k < usable;
-    const auto finish = [&](int m) {
-      const bool in = tid < m && (!by_count || tid < k);
-      const float l = in ? own_l[tid] : -INFINITY;
-      const double w = in ? (double)weight(l) : 0.;
-      double kept_mass;
-      const double before = block_scan_inclusive(w, dpart, kept_mass) - w;
-      const double target = p < 1.f ? p * (by_count ? kept_mass : Z) : INFINITY;
-      Best best = {-INFINITY, INT32_MAX};
-      if (in && (tid == 0 || before < target) && heavy_enough(l))
-        best = {key_of(l, a.noise[row * a.noise_stride + own_i[tid]]), own_i[tid]};
-      const Best won = block_best(best, part);
-      if (in && best.index == won.index) answer(won.index, l);
-    };
+    const bool by_count = k < usable, by_mass = p < 1.f;
 
-    fetch();
-    int4 bins = find_bins(!by_count, by_count ? (double)k : (double)p * Z, 0., true);
-    if ((by_count || p < 1.f) && reached && bins.w <= kCandidates) {
-      const int m = gather(-INFINITY, 0, bins.y);
+    // ---- how far down the threads' greatest reach the limit, if they do
+    int reach;
+    {
+      if (tid == 0) sh_bin = kBins;
+      const uint32_t c0 = all[2 * tid], c1 = all[2 * tid + 1];
+      double v0 = c0, v1 = c1;
+      if (!by_count) {  // the least mass they can have (nothing for the last, open bin)
+        const auto edge = [&](int b) { return (double)weight(top - b / bins_per_logit) * (1. - 1e-4); };
+        v0 *= edge(2 * tid + 1);
+        v1 *= 2 * tid + 1 == kBins - 1 ? 0. : edge(2 * tid + 2);
+      }
+      const double want = by_count ? (double)k : (double)p * Z;
+      double sum;
+      const double through = block_scan_inclusive(v0 + v1, dpart, sum);
+      if (through - v1 >= want) atomicMin(&sh_bin, 2 * tid);
+      if (through >= want) atomicMin(&sh_bin, 2 * tid + 1);
+      __syncthreads();
+      reach = sh_bin;
+    }
+    if ((by_count || by_mass) && reach < kBins - 1) {
+      // a compare first, one step too low, and the bins' exact test for what passes
+      const float edge = top - (reach + 2) / bins_per_logit;
+      const int m = gather([&](float l) { return l >= edge && bin_of(l) <= reach; });
       if (m <= kCandidates) {
-        if (rank == 0) finish(m);
+        if (rank != 0) return;
+        // ---- all limits on the ranked list
+        const bool in = tid < m && (!by_count || tid < k);
+        const float l = in ? own_l[tid] : -INFINITY;
+        const double w = in ? (double)weight(l) : 0.;
+        double kept_mass;
+        const double before = block_scan_inclusive(w, dpart, kept_mass) - w;
+        const double target = by_mass ? p * (by_count ? kept_mass : Z) : INFINITY;
+        Best best = {-INFINITY, INT32_MAX};
+        if (in && (tid == 0 || before < target) && heavy_enough(l))
+          best = {key_of(l, a.noise[row * a.noise_stride + own_i[tid]]), own_i[tid]};
+        const Best won = block_best(best, part);
+        if (in && best.index == won.index) answer(won.index, l);
         return;
       }
     }
 
-    // ---- cuts by narrowing
-    cluster.sync();  // every block has read the pooled histogram, which is cleared next
-    for (int limit = 0; limit < 2; ++limit) {  // top_k, then top_p
-      const bool by_mass = limit == 1;
-      if (by_mass ? !(p < 1.f) : !by_count) continue;
-      double want = k, above = 0.;
-      if (by_mass) {
-        double mass = Z;
-        if (by_count) {  // what top_k left
-          float left = 0.f;
-          each([&](float l, int) { left += weight(l); });
-          mass = over_cluster(block_sum(left), 0., add).x;
-        }
-        want = p * mass;
+    // Count and mass of the tokens that `takes(l, i)`.
+    const auto measure = [&](auto takes) {
+      float m = 0.f;
+      int c = 0;
+      each([&](float l, int i) {
+        if (takes(l, i)) m += weight(l), ++c;
+      });
+      return over_cluster(block_sum(m), block_sum(c), add);
+    };
+    // Strikes out what a limit does not keep: top_k (mass = false) or top_p with `want` of the mass
+    const auto strike = [&](bool mass, double want) {
+      // the least key that is kept, if only in part, is in (below, at]
+      uint32_t at = order_key(top), below = order_key(-FLT_MAX) - 1;
+      double above = 0.;                    // count or mass over `at`
+      int over_at = 0, over_below = usable; // counts over `at` and over `below`
+      while (at - below > 1 && over_below - over_at > kCandidates) {
+        const uint32_t mid = below + (at - below) / 2;
+        const double2 over = measure([&](float l, int) { return order_key(l) > mid; });
+        const double v = mass ? over.x : over.y;
+        if (v < want) at = mid, above = v, over_at = (int)over.y;
+        else below = mid, over_below = (int)over.y;
       }
-      hi = top;
-      key_scale = 0;
-      float least = -INFINITY;
-      int above_count = 0;
-      for (int level = 0;; ++level) {
-        // histogram of the logits from `least` to hi
-        for (int b = tid; b < kBins; b += kSliceThreads) hist[b] = total[b] = 0;
-        cluster.sync();
-        each([&](float l, int) {
-          if (l >= least && l <= hi) atomicAdd(&hist[bin_of(l)], 1u);
+      if (at - below > 1) {
+        const int m = gather([&](float l) {
+          const uint32_t key = order_key(l);
+          return key > below && key <= at;
         });
+        if (rank == 0) {
+          const float l = tid < m ? own_l[tid] : -INFINITY;
+          const double w = tid >= m ? 0. : mass ? (double)weight(l) : 1.;
+          double unused;
+          const double before = above + block_scan_inclusive(w, dpart, unused) - w;
+          const int kept = max((int)block_sum(tid < m && before < want ? 1. : 0.), 1);
+          const float cut = own_l[kept - 1];
+          const int ties = (int)block_sum(tid < kept && l == cut ? 1. : 0.);
+          if (tid < ranks) {
+            *cluster.map_shared_rank(&sh_cut, tid) = cut;
+            *cluster.map_shared_rank(&sh_ties, tid) = ties;
+          }
+        }
+        cluster.sync();
+      } else {  // ties of one key: as many as the limit still takes
+        const float cut = key_value(at);
+        if (tid == 0) {
+          const double w = mass ? weight(cut) : 1.;
+          sh_cut = cut;
+          sh_ties = w > 0. ? (int)fmin(ceil((want - above) / w), 2147483647.) : 1;
+        }
         __syncthreads();
-        pool_hist();
-        cluster.sync();
-        fetch();
-        bins = find_bins(by_mass, by_mass ? want : want - above_count, by_mass ? above : 0.,
-                         level == 0);
-        if (by_mass && level > 0 && bins.x == 0 && bins.y == bin_of(least)) {
-          // the bounds leave every bin (coarse ones, or few values many times): the exact mass
-          // of the upper half of the bins decides between the halves, and neither is empty,
-          // since hi is in the first bin and the least value in the last
-          const int half = bins.y / 2;
-          float up = 0.f;
-          int count = 0;
-          each([&](float l, int) {
-            if (l < least || l > hi || bin_of(l) > half) return;
-            up += weight(l);
-            ++count;
-          });
-          const double2 upper = over_cluster(block_sum(up), block_sum(count), add);
-          if (above + upper.x >= want) bins.y = half, bins.w = (int)upper.y;
-          else bins.x = half + 1, bins.z = (int)upper.y;
-        }
-        const int members = bins.w - bins.z;
-        above_count += bins.z;
-        // mass above the bins; range of the values in them
-        float up = 0.f, low = INFINITY, high = -INFINITY;
-        each([&](float l, int) {
-          if (l < least || l > hi) return;
-          const int b = bin_of(l);
-          if (b < bins.x) up += weight(l);
-          else if (b <= bins.y) low = fminf(low, l), high = fmaxf(high, l);
-        });
-        above += over_cluster(block_sum(up), 0., add).x;
-        const double2 range = over_cluster(block_max(-low), block_max(high), most);
-        low = -(float)range.x;
-        high = (float)range.y;
-        if (low == high || level >= 64) {  // ties: as many as the limit still takes
-          if (tid == 0) {
-            const double w = weight(low);
-            const double takes = !by_mass ? want - above_count
-                                 : w > 0. ? ceil((want - above) / w) : 1.;
-            sh_cut = low;
-            sh_ties = (int)fmin(fmax(takes, above_count ? 0. : 1.), (double)members);
-          }
-          __syncthreads();
-          break;
-        }
-        if (members <= kCandidates) {
-          const int m = gather(least, bins.x, bins.y);
-          if (rank == 0) {
-            const float l = tid < m ? own_l[tid] : -INFINITY;
-            const double w = tid < m ? (double)weight(l) : 0.;
-            double unused;
-            const double before = above + block_scan_inclusive(w, dpart, unused) - w;
-            const bool in = tid < m && (by_mass ? before < want || (above_count == 0 && tid == 0)
-                                                : above_count + tid < want);
-            const int kept = max((int)block_sum(in ? 1. : 0.), 1);
-            const float cut = own_l[kept - 1];
-            const int ties = (int)block_sum(tid < kept && l == cut ? 1. : 0.);
-            if (tid < ranks) {
-              *cluster.map_shared_rank(&sh_cut, tid) = cut;
-              *cluster.map_shared_rank(&sh_ties, tid) = ties;
-            }
-          }
-          cluster.sync();
-          break;
-        }
-        // narrower: the values between low and high
-        least = low;
-        hi = high;
-        key_scale = ((uint64_t)kBins << 32) / ((uint64_t)order_key(high) - order_key(low) + 1);
       }
-      // strike out what is below the cut, and the ties past the last one kept
       const float cut = sh_cut;
       const int ties = sh_ties;
       int mine = 0;
@@ -698,65 +679,40 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
         if (out) slice[i] = from_f32<L>(-INFINITY);
       }
       __syncthreads();
+    };
+
+    double want = k;  // of the one limit left: a rank, or a mass
+    bool left = by_count || by_mass;
+    if (by_mass) {
+      double mass = Z;
+      if (by_count) {
+        strike(false, k);
+        mass = measure([](float, int) { return true; }).x;
+      }
+      want = fmax(p * mass, 1e-30);  // the greatest is always kept
+    }
+    if (left) {
+      float bound_l = -INFINITY, l;
+      int bound_i = 0;
+      for (int turns = 0; turns < kDraws; ++turns) {
+        const Best won = draw(bound_l, bound_i, l);
+        const double2 over = measure([&](float x, int i) {
+          return x > l || (x == l && first + i < won.index);
+        });
+        if ((by_mass ? over.x : over.y) < want) {
+          if (rank == 0 && tid == 0) answer(won.index, l);
+          return;
+        }
+        bound_l = l;
+        bound_i = won.index;
+      }
+      strike(by_mass, want);
     }
   }
 
-  // ---- the best of what is left
-  Best best = {-INFINITY, INT32_MAX};
-  float best_l = 0.f;
-  if (!hot) {
-    each([&](float l, int i) {
-      if (l == top && first + i < best.index) best = {l, first + i}, best_l = l;
-    });
-  } else {
-    // The logarithm in full only where its approximation comes within 1e-3 of the best so far
-    // (t within 2^-22 of |t| by the reciprocal's rounding, below that for |t| up to 2000).
-    const float inv = 1.f / div;
-    const float sure = least_weight > 0.f ? (top_t + logf(least_weight)) - 1e-3f : -INFINITY;
-    const auto consider = [&](float l, int i, float e) {
-      const float t = l * inv;
-      if (t - __logf(e) < best.value - 1e-3f - fabsf(t) * 5e-7f) return;
-      const Best b = {key_of(l, e), first + i};
-      if (b.value > best.value || (b.value == best.value && b.index < best.index)) best = b, best_l = l;
-    };
-    if (least_weight > 0.f) {
-      each([&](float l, int i) {
-        if (l * inv + fabsf(l * inv) * 5e-7f < sure || !heavy_enough(l)) return;
-        consider(l, i, noise[i]);
-      });
-    } else {
-      for (int i0 = tid; i0 < n; i0 += 8 * kSliceThreads) {
-        float e[8], l[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int i = i0 + j * kSliceThreads;
-          l[j] = i < n ? to_f32<L>(slice[i]) : -INFINITY;
-          e[j] = l[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (l[j] > -INFINITY) consider(l[j], i0 + j * kSliceThreads, e[j]);
-      }
-    }
-  }
-  const Best own = best;
-  best = block_best(best, part);
-  if (own.index == best.index && best.index < V) {
-    cluster.map_shared_rank(cluster_best, 0)[rank] = best;
-    cluster.map_shared_rank(cluster_l, 0)[rank] = best_l;
-  } else if (tid == 0 && best.index >= V) {  // nothing of this slice is left
-    cluster.map_shared_rank(cluster_best, 0)[rank] = best;
-  }
-  cluster.sync();
-  if (rank == 0 && tid == 0) {
-    int who = 0;
-    for (int r = 1; r < ranks; ++r)
-      if (cluster_best[r].value > cluster_best[who].value ||
-          (cluster_best[r].value == cluster_best[who].value &&
-           cluster_best[r].index < cluster_best[who].index))
-        who = r;
-    answer(cluster_best[who].index, cluster_l[who]);
-  }
+  float l;
+  const Best won = draw(-INFINITY, 0, l);
+  if (rank == 0 && tid == 0) answer(won.index, l);
 }
 
 template <typename L>
