@@ -1,6 +1,7 @@
 // tr_residual_norm: the norm after a block, its gate, the scaled residual add and the norm
 // before the next block, in one pass over the row.
 #include <algorithm>
+#include <type_traits>
 
 #include "serve_util.cuh"
 
@@ -21,174 +22,216 @@ struct NormArgs {
   float eps, residual_scale, branch_scale;
 };
 
-// Sum over the G threads of a row.  Rows of more than a warp go through shared memory, with one
-// barrier a call: successive calls alternate between the two buffers, so a thread may write the
-// next sums while others still read these.
-template <int G>
-__device__ __forceinline__ float row_sum(float v, float (*part)[32], int& turn) {
-  v = warp_sum(v);
-  if constexpr (G > 32) {
-    const int lane = threadIdx.x & 31;
-    float* p = part[turn & 1];
+// Sums of x and y over the threads of a row: a warp (ROW_WARP) or the block.  Rows of more than
+// a warp go through shared memory, with one barrier a call: successive calls alternate between
+// the two buffers, so a thread may write the next sums while others still read these.
+template <bool ROW_WARP>
+__device__ __forceinline__ float2 row_sum(float x, float y, float2 (*part)[32], int& turn) {
+  x = warp_sum(x);
+  y = warp_sum(y);
+  if constexpr (!ROW_WARP) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    float2* p = part[turn & 1];
     ++turn;
-    if (lane == 0) p[threadIdx.x >> 5] = v;
+    if (lane == 0) p[threadIdx.x >> 5] = make_float2(x, y);
     __syncthreads();
-    v = warp_sum(lane < G / 32 ? p[lane] : 0.f);
+    const float2 v = lane < warps ? p[lane] : make_float2(0.f, 0.f);
+    x = warp_sum(v.x);
+    y = warp_sum(v.y);
   }
-  return v;
+  return make_float2(x, y);
+}
+
+// N vectors of V elements as they lie in memory; elements past the width are zeros
+template <typename T, int N, int V>
+struct Row {
+  static constexpr int WORDS = V * sizeof(T) >= 16 ? V * sizeof(T) / 16 : 1;
+  using Word = typename std::conditional<V == 8, uint4, T>::type;
+  Word w[N][WORDS];
+
+  __device__ __forceinline__ void load(const T* p, int t, int threads, int width, bool held) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * threads + t) * V;
+      const bool in = held && c < width;
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) {
+        if constexpr (V == 8)
+          w[i][j] = in ? reinterpret_cast<const uint4*>(p + c)[j] : make_uint4(0, 0, 0, 0);
+        else
+          w[i][j] = in ? p[c] : from_f32<T>(0.f);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(int i, float (&f)[V]) const {
+    if constexpr (V == 1) f[0] = to_f32<T>(w[i][0]);
+    else load8<T>(reinterpret_cast<const T*>(w[i]), f);
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void get_vector(const T* p, float (&f)[V]) {
+  if constexpr (V == 1) f[0] = to_f32<T>(p[0]);
+  else load8<T>(p, f);
 }
 
 // f <- N(f) * weight + bias over one row; entries past the width hold zeros and stay out of the
 // sums.  The mean is taken out before the squares are summed: sums of squares about zero would
 // cancel where the mean is large against the spread.  What the first mean is off by (fp32: up to
 // 2^-24 of it and the sum's error) is the mean of the differences, summed next to their squares.
-template <typename E, bool LAYER, int G, int N, int V>
-__device__ __forceinline__ void norm_row(float (&f)[N * V], const E* weight, const E* bias,
-                                         int width, float eps, float (*part)[32], int& turn) {
-  const int t = G > 32 ? threadIdx.x : threadIdx.x & 31;
-  const float inv_width = 1.f / (float)width;
+template <typename E, bool LAYER, bool ROW_WARP, int N, int V>
+__device__ __forceinline__ void norm_row(float (&f)[N][V], const E* weight, const E* bias, int t,
+                                         int threads, int width, float inv_width, float eps,
+                                         float2 (*part)[32], int& turn) {
   float mean = 0.f;
   if constexpr (LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < N * V; ++i) s += f[i];
-    mean = row_sum<G>(s, part, turn) * inv_width;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += f[i][j];
+    mean = row_sum<ROW_WARP>(s, 0.f, part, turn).x * inv_width;
   }
   float s = 0.f, d = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if ((i * G + t) * V < width) {
+    const float m = (i * threads + t) * V < width ? mean : 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        f[i * V + j] -= mean;
-        if constexpr (LAYER) d += f[i * V + j];
-        s = fmaf(f[i * V + j], f[i * V + j], s);
+    for (int j = 0; j < V; ++j) {
+      if constexpr (LAYER) {
+        f[i][j] -= m;
+        d += f[i][j];
       }
+      s = fmaf(f[i][j], f[i][j], s);
     }
   }
-  s = row_sum<G>(s, part, turn) * inv_width;
+  const float2 sums = row_sum<ROW_WARP>(s, d, part, turn);
+  s = sums.x * inv_width;
   if constexpr (LAYER) {
-    d = row_sum<G>(d, part, turn) * inv_width;
+    d = sums.y * inv_width;
     s = fmaf(-d, d, s);
   }
   const float r = rsqrtf(s + eps);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * V;
+    const int c = (i * threads + t) * V;
     if (c >= width) continue;
-    if constexpr (V == 8) {
-      float w[8];
-      load8<E>(weight + c, w);
+    float w[V];
+    get_vector<E, V>(weight + c, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[i * 8 + j] = (f[i * 8 + j] - d) * (r * w[j]);
-      if (bias) {
-        load8<E>(bias + c, w);
+    for (int j = 0; j < V; ++j) f[i][j] = (LAYER ? f[i][j] - d : f[i][j]) * (r * w[j]);
+    if (bias) {
+      get_vector<E, V>(bias + c, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[i * 8 + j] += w[j];
-      }
-    } else {
-      f[i] = (f[i] - d) * (r * to_f32<E>(weight[c])) + (bias ? to_f32<E>(bias[c]) : 0.f);
+      for (int j = 0; j < V; ++j) f[i][j] += w[j];
     }
   }
 }
 
-template <typename T, int G, int N, int V>
-__device__ __forceinline__ void load_row(const T* p, int width, float (&f)[N * V]) {
-  const int t = G > 32 ? threadIdx.x : threadIdx.x & 31;
+template <typename E, int N, int V>
+__device__ __forceinline__ void store_row(E* p, int t, int threads, int width,
+                                          const float (&f)[N][V]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * V;
-    if constexpr (V == 8) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < width) load8<T>(p + c, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[i * 8 + j] = v[j];
-    } else {
-      f[i] = c < width ? to_f32<T>(p[c]) : 0.f;
-    }
-  }
-}
-template <typename E, int G, int N, int V>
-__device__ __forceinline__ void store_row(E* p, int width, const float (&f)[N * V]) {
-  const int t = G > 32 ? threadIdx.x : threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * V;
+    const int c = (i * threads + t) * V;
     if (c >= width) continue;
-    if constexpr (V == 8) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = f[i * 8 + j];
-      store8<E>(p + c, v);
-    } else {
-      p[c] = from_f32<E>(f[i]);
-    }
+    if constexpr (V == 8) store8<E>(p + c, f[i]);
+    else p[c] = from_f32<E>(f[i][0]);
   }
 }
 
-// G threads hold a row in registers as N vectors of V elements each (G = 32: a warp per row, 8
-// rows a block; else a block per row), so y and h are read once and both outputs written once
-// whatever the norms need.
-template <typename E, typename Y, bool LAYER, int G, int N, int V>
-__global__ void __launch_bounds__(G > 32 ? G : 256) residual_norm_kernel(const NormArgs a) {
-  __shared__ float part[2][32];
+// A row lies in the registers of its threads (a warp, 8 rows a block; or the block) as N vectors
+// of V elements each, so y and h are read once and both outputs written once whatever the
+// norms need.  A block takes every gridDim.x-th row; where the registers hold it (one vector a
+// thread) it loads the next row before it works on this one, whose sums each cost a barrier,
+// else other blocks of the SM cover them.  The weights come from L1.  Bound by memory.
+template <typename E, typename Y, bool LAYER, bool ROW_WARP, int N, int V, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) residual_norm_kernel(const NormArgs a) {
+  constexpr bool AHEAD = N * V <= 8;
+  __shared__ float2 part[2][32];
   int turn = 0;
-  const int64_t rows_per_block = G > 32 ? 1 : 8;
-  for (int64_t row = blockIdx.x * rows_per_block + (G > 32 ? 0 : threadIdx.x >> 5); row < a.tokens;
-       row += gridDim.x * rows_per_block) {
-    float f[N * V], g[N * V];
-    load_row<E, G, N, V>(static_cast<const E*>(a.h) + row * a.h_stride, a.width, g);
-    if (a.y) {
-      load_row<Y, G, N, V>(static_cast<const Y*>(a.y) + row * a.y_stride, a.width, f);
+  const int t = ROW_WARP ? threadIdx.x & 31 : threadIdx.x, threads = ROW_WARP ? 32 : blockDim.x;
+  const int rows_at_once = ROW_WARP ? THREADS / 32 : 1;
+  const int64_t first = (int64_t)blockIdx.x * rows_at_once + (ROW_WARP ? threadIdx.x >> 5 : 0);
+  const int64_t stride = (int64_t)gridDim.x * rows_at_once;
+  const float inv_width = 1.f / (float)a.width;
+  const E *h = static_cast<const E*>(a.h), *gate = static_cast<const E*>(a.gate);
+  const Y* y = static_cast<const Y*>(a.y);
+  Row<E, N, V> next_h, next_gate;
+  Row<Y, N, V> next_y;
+  const auto fetch = [&](int64_t row) {
+    const bool held = row < a.tokens;
+    next_h.load(h + row * a.h_stride, t, threads, a.width, held);
+    next_y.load(y + row * a.y_stride, t, threads, a.width, held && y);
+    next_gate.load(gate + row * a.gate_stride, t, threads, a.width, held && gate);
+  };
+  if constexpr (AHEAD) fetch(first);
+  for (int64_t row = first; row < a.tokens; row += stride) {
+    if constexpr (!AHEAD) fetch(row);
+    const Row<E, N, V> row_h = next_h, row_gate = next_gate;
+    const Row<Y, N, V> row_y = next_y;
+    if constexpr (AHEAD) fetch(row + stride);
+    float f[N][V], g[V];
+    if (y) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) row_y.get(i, f[i]);
       if (a.post)
-        norm_row<E, LAYER, G, N, V>(f, static_cast<const E*>(a.post),
-                                    static_cast<const E*>(a.post_bias), a.width, a.eps, part, turn);
+        norm_row<E, LAYER, ROW_WARP, N, V>(f, static_cast<const E*>(a.post),
+                                          static_cast<const E*>(a.post_bias), t, threads, a.width,
+                                          inv_width, a.eps, part, turn);
 #pragma unroll
-      for (int i = 0; i < N * V; ++i) g[i] *= a.residual_scale;
-      if (a.gate) {
-        float w[N * V];
-        load_row<E, G, N, V>(static_cast<const E*>(a.gate) + row * a.gate_stride, a.width, w);
+      for (int i = 0; i < N; ++i) {
+        if (gate) {
+          row_gate.get(i, g);
 #pragma unroll
-        for (int i = 0; i < N * V; ++i) f[i] *= w[i];
+          for (int j = 0; j < V; ++j) f[i][j] *= g[j];
+        }
+        row_h.get(i, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          f[i][j] = fmaf(a.branch_scale, f[i][j], a.residual_scale * g[j]);
       }
+      store_row<E, N, V>(static_cast<E*>(a.h_out) + row * a.width, t, threads, a.width, f);
+    } else {
 #pragma unroll
-      for (int i = 0; i < N * V; ++i) g[i] = fmaf(a.branch_scale, f[i], g[i]);
-      store_row<E, G, N, V>(static_cast<E*>(a.h_out) + row * a.width, a.width, g);
+      for (int i = 0; i < N; ++i) row_h.get(i, f[i]);
     }
     if (a.pre) {
-      norm_row<E, LAYER, G, N, V>(g, static_cast<const E*>(a.pre),
-                                  static_cast<const E*>(a.pre_bias), a.width, a.eps, part, turn);
-      store_row<E, G, N, V>(static_cast<E*>(a.x_out) + row * a.width, a.width, g);
+      norm_row<E, LAYER, ROW_WARP, N, V>(f, static_cast<const E*>(a.pre),
+                                        static_cast<const E*>(a.pre_bias), t, threads, a.width,
+                                        inv_width, a.eps, part, turn);
+      store_row<E, N, V>(static_cast<E*>(a.x_out) + row * a.width, t, threads, a.width, f);
     }
   }
 }
 
-template <typename E, typename Y, bool LAYER, int G, int N, int V>
+// THREADS: the most a block has; BLOCKS: the blocks of that size that an SM holds
+template <typename E, typename Y, bool LAYER, bool ROW_WARP, int N, int V, int THREADS, int BLOCKS>
 static int launch_norm(const NormArgs& a, void* stream) {
-  const int64_t rows_per_block = G > 32 ? 1 : 8;
-  const int64_t blocks = (a.tokens + rows_per_block - 1) / rows_per_block;
-  const int threads = G > 32 ? G : 256;
-  const int64_t most = (int64_t)serve_sms() * (2048 / threads);
-  residual_norm_kernel<E, Y, LAYER, G, N, V>
+  const int vectors = (a.width + V - 1) / V;
+  const int threads = ROW_WARP ? THREADS : ((vectors + N - 1) / N + 31) / 32 * 32;
+  const int64_t rows_at_once = ROW_WARP ? THREADS / 32 : 1;
+  const int64_t blocks = (a.tokens + rows_at_once - 1) / rows_at_once;
+  const int64_t most = (int64_t)serve_sms() * (THREADS * BLOCKS / threads);
+  residual_norm_kernel<E, Y, LAYER, ROW_WARP, N, V, THREADS, BLOCKS>
       <<<(unsigned)std::min(blocks, most), threads, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return serve_launched("tr_residual_norm");
 }
 
 template <typename E, typename Y, bool LAYER>
 static int pick_norm(const NormArgs& a, bool wide, void* stream) {
-  if (wide) {
-    const int vectors = a.width / 8;
-    if (vectors <= 64) return launch_norm<E, Y, LAYER, 32, 2, 8>(a, stream);
-    if (vectors <= 128) return launch_norm<E, Y, LAYER, 128, 1, 8>(a, stream);
-    if (vectors <= 256) return launch_norm<E, Y, LAYER, 256, 1, 8>(a, stream);
-    if (vectors <= 512) return launch_norm<E, Y, LAYER, 512, 1, 8>(a, stream);
-    if (vectors <= 1024) return launch_norm<E, Y, LAYER, 512, 2, 8>(a, stream);
-    return launch_norm<E, Y, LAYER, 1024, 4, 8>(a, stream);
+  if (wide) {  // widths to 512 a warp a row; then vectors a thread by what a block holds
+    if (a.width <= 256) return launch_norm<E, Y, LAYER, true, 1, 8, 256, 4>(a, stream);
+    if (a.width <= 512) return launch_norm<E, Y, LAYER, true, 2, 8, 256, 3>(a, stream);
+    if (a.width <= 1024) return launch_norm<E, Y, LAYER, true, 4, 8, 256, 2>(a, stream);
+    if (a.width <= 4096) return launch_norm<E, Y, LAYER, false, 2, 8, 256, 4>(a, stream);
+    if (a.width <= 8192) return launch_norm<E, Y, LAYER, false, 2, 8, 512, 2>(a, stream);
+    if (a.width <= 16384) return launch_norm<E, Y, LAYER, false, 4, 8, 512, 1>(a, stream);
+    return launch_norm<E, Y, LAYER, false, 4, 8, 1024, 1>(a, stream);
   }
-  if (a.width <= 256) return launch_norm<E, Y, LAYER, 32, 8, 1>(a, stream);
-  if (a.width <= 2048) return launch_norm<E, Y, LAYER, 256, 8, 1>(a, stream);
-  if (a.width <= 8192) return launch_norm<E, Y, LAYER, 1024, 8, 1>(a, stream);
-  return launch_norm<E, Y, LAYER, 1024, 32, 1>(a, stream);
+  if (a.width <= 256) return launch_norm<E, Y, LAYER, true, 8, 1, 256, 4>(a, stream);
+  if (a.width <= 4096) return launch_norm<E, Y, LAYER, false, 8, 1, 512, 2>(a, stream);
+  return launch_norm<E, Y, LAYER, false, 32, 1, 1024, 1>(a, stream);
 }
 
 template <typename E, typename Y>

@@ -3,6 +3,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "serve_util.cuh"
 
@@ -260,9 +261,29 @@ struct RowSums {  // one value or two per block of the cluster, in every block
   double v[2][8][2];
 };
 
+// The greatest of the logits in a 16-byte vector (NaN aside), and NaN made -inf in it.
 template <typename L>
-__device__ __forceinline__ L not_nan(L x) {
-  return to_f32<L>(x) == to_f32<L>(x) ? x : from_f32<L>(-INFINITY);
+__device__ __forceinline__ float settle(uint4& x) {
+  using P = typename std::conditional<std::is_same<L, __half>::value, __half2, __nv_bfloat162>::type;
+  P* w = reinterpret_cast<P*>(&x);
+  const bool clean = __hbeq2(w[0], w[0]) && __hbeq2(w[1], w[1]) && __hbeq2(w[2], w[2]) &&
+                     __hbeq2(w[3], w[3]);
+  if (!clean) {
+    L* e = reinterpret_cast<L*>(&x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (__hisnan(e[j])) e[j] = from_f32<L>(-INFINITY);
+  }
+  const P m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+  return fmaxf(to_f32<L>(m.x), to_f32<L>(m.y));
+}
+template <>
+__device__ __forceinline__ float settle<float>(uint4& x) {
+  float* e = reinterpret_cast<float*>(&x);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (isnan(e[j])) e[j] = -INFINITY;
+  return fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
 }
 
 template <typename L>
@@ -372,11 +393,7 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
         for (int j = 0; j < W; ++j)
           e[j] = v * W + j < n ? logits[v * W + j] : from_f32<L>(-INFINITY);
       }
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        e[j] = not_nan(e[j]);
-        greatest = fmaxf(greatest, to_f32<L>(e[j]));
-      }
+      greatest = fmaxf(greatest, settle<L>(x));
       slice_raw[v] = x;
     }
   }
@@ -418,14 +435,21 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
 
   float z = 0.f;
   int finite = 0;
+#pragma unroll 2
   for (int v = tid; v < vectors; v += kSliceThreads) {
     const uint4 x = slice_raw[v];
     const L* e = reinterpret_cast<const L*>(&x);
+    float w[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float l = to_f32<L>(e[j]);
-      z += weight(l);
-      finite += l > -INFINITY;
+    for (int j = 0; j < W; ++j) w[j] = weight(to_f32<L>(e[j]));
+#pragma unroll
+    for (int d = W / 2; d; d /= 2)
+#pragma unroll
+      for (int j = 0; j < d; ++j) w[j] += w[j + d];
+    z += w[0];
+    if (k < V) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) finite += to_f32<L>(e[j]) > -INFINITY;
     }
   }
   if (limited && greatest > -INFINITY) atomicAdd(&hist[bin_of(greatest)], 1u);
@@ -438,7 +462,7 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   }
   const double2 both = over_cluster(zs, fs, add);
   const double Z = both.x;
-  const int usable = (int)both.y;
+  const int usable = k < V ? (int)both.y : V;  // where top_k is off, not asked for
   const float log_z = logf((float)Z);
   const auto answer = [&](int index, float l) {
     a.tokens[row] = index;

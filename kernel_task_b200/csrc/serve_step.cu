@@ -206,50 +206,86 @@ static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, si
 
 // ---- tr_append_kv
 struct AppendArgs {
-  const void* src[2];
-  void* dst[2];
-  int64_t token_stride[2], head_stride[2];
+  const void* k;
+  const void* v;
+  void* k_pages;
+  void* v_pages;
+  int64_t k_token, k_head, v_token, v_head;  // source strides
   const int64_t* slots;
   int64_t tokens, slots_end;
   int heads, dim, page;
+  int page_shift;              // of a page size that is a power of two, else -1
+  int step_tokens, step_rest;  // what a grid's stride of vectors is in tokens and the rest
 };
 
 // One thread per 8 elements (V = 8, 16-byte stores) or per element (V = 1, when a source row is
-// not 16-byte aligned).  blockIdx.y: keys or values.  Bound by memory at large sizes (a source
-// element read, a pool element written), by the launch at small ones.
+// not 16-byte aligned) of both keys and values; four of them at a time, so that their slots,
+// then their sources, are in flight together.  The token and head of a vector are divided out
+// once and carried on.  Bound by memory at large sizes, by the launch at small ones.
 template <typename S, typename E, int V>
 __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs a) {
-  const int which = blockIdx.y;
-  const S* src = static_cast<const S*>(a.src[which]);
-  E* dst = static_cast<E*>(a.dst[which]);
+  constexpr int U = 4;
   const int per_head = a.dim / V, per_token = a.heads * per_head;
-  const int64_t n = a.tokens * per_token;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / per_token;
-    const int rest = (int)(i - t * per_token), h = rest / per_head, d = (rest - h * per_head) * V;
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.slots_end) continue;
-    const int64_t page = slot / a.page;
-    const S* from = src + t * a.token_stride[which] + h * a.head_stride[which] + d;
-    E* to = dst + ((page * a.heads + h) * a.page + (slot - page * a.page)) * a.dim + d;
-    if constexpr (V == 8) {
-      float f[8];
-      load8<S>(from, f);
-      store8<E>(to, f);
-    } else {
-      *to = from_f32<E>(to_f32<S>(*from));
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  int64_t t = i / per_token;
+  int rest = (int)(i - t * per_token);
+  while (t < a.tokens) {
+    int64_t token[U], slot[U];
+    int in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      token[u] = t;
+      in[u] = rest;
+      slot[u] = t < a.tokens ? a.slots[t] : -1;
+      t += a.step_tokens;
+      rest += a.step_rest;
+      if (rest >= per_token) rest -= per_token, ++t;
+    }
+    float f[U][2][V];
+    int64_t to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      to[u] = -1;
+      if (slot[u] < 0 || slot[u] >= a.slots_end) continue;
+      const int h = in[u] / per_head, d = (in[u] - h * per_head) * V;
+      const int64_t page = a.page_shift >= 0 ? slot[u] >> a.page_shift : slot[u] / a.page;
+      to[u] = ((page * a.heads + h) * a.page + (slot[u] - page * a.page)) * a.dim + d;
+      const S* k = static_cast<const S*>(a.k) + token[u] * a.k_token + h * a.k_head + d;
+      const S* v = static_cast<const S*>(a.v) + token[u] * a.v_token + h * a.v_head + d;
+      if constexpr (V == 8) {
+        load8<S>(k, f[u][0]);
+        load8<S>(v, f[u][1]);
+      } else {
+        f[u][0][0] = to_f32<S>(*k);
+        f[u][1][0] = to_f32<S>(*v);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (to[u] < 0) continue;
+      E* k = static_cast<E*>(a.k_pages) + to[u];
+      E* v = static_cast<E*>(a.v_pages) + to[u];
+      if constexpr (V == 8) {
+        store8<E>(k, f[u][0]);
+        store8<E>(v, f[u][1]);
+      } else {
+        *k = from_f32<E>(f[u][0][0]);
+        *v = from_f32<E>(f[u][1][0]);
+      }
     }
   }
 }
 
 template <typename S, typename E>
-static int launch_append(const AppendArgs& a, bool wide, void* stream) {
-  const int64_t n = a.tokens * a.heads * (a.dim / (wide ? 8 : 1));
-  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)serve_sms() * 16), 2);
+static int launch_append(AppendArgs a, bool wide, void* stream) {
+  const int64_t per_token = (int64_t)a.heads * (a.dim / (wide ? 8 : 1));
+  const int64_t n = a.tokens * per_token;
+  const int64_t blocks = std::min<int64_t>((n + 255) / 256, (int64_t)serve_sms() * 8);
+  a.step_tokens = (int)(blocks * 256 / per_token);
+  a.step_rest = (int)(blocks * 256 % per_token);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (wide) append_kv_kernel<S, E, 8><<<grid, 256, 0, s>>>(a);
-  else append_kv_kernel<S, E, 1><<<grid, 256, 0, s>>>(a);
+  if (wide) append_kv_kernel<S, E, 8><<<(unsigned)blocks, 256, 0, s>>>(a);
+  else append_kv_kernel<S, E, 1><<<(unsigned)blocks, 256, 0, s>>>(a);
   return serve_launched("tr_append_kv");
 }
 
@@ -347,7 +383,7 @@ extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_hea
     set_error("tr_append_kv: null pointer");
     return TR_ERR_INVALID;
   }
-  const int sb = element_bytes(src_dtype), db = element_bytes(dtype);
+  const int sb = element_bytes(src_dtype);
   if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) {
     set_error("tr_append_kv: the pools must be 16-byte aligned");
     return TR_ERR_ALIGN;
@@ -356,9 +392,9 @@ extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_hea
     set_error("tr_append_kv: a pointer is not aligned to its elements");
     return TR_ERR_ALIGN;
   }
-  AppendArgs a = {{k, v}, {k_pages, v_pages}, {k_token_stride, v_token_stride},
-                  {k_head_stride, v_head_stride}, slots, tokens, pages * page_size, kv_heads,
-                  head_dim, page_size};
+  AppendArgs a = {k, v, k_pages, v_pages, k_token_stride, k_head_stride, v_token_stride,
+                  v_head_stride, slots, tokens, pages * page_size, kv_heads, head_dim, page_size,
+                  page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), 0, 0};
   const bool wide = head_dim % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) &&
                     !((k_token_stride * sb | k_head_stride * sb | v_token_stride * sb |
                        v_head_stride * sb) & 15);
@@ -368,6 +404,5 @@ extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_hea
     return launch_append<float, __nv_bfloat16>(a, wide, stream);
   }
   if (dtype == TR_F16) return launch_append<__half, __half>(a, wide, stream);
-  (void)db;
   return launch_append<__nv_bfloat16, __nv_bfloat16>(a, wide, stream);
 }
