@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "serve_util.cuh"
+#include "tc_util.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -32,91 +33,133 @@ constexpr int kStepThreads = 1024;
 
 __device__ __forceinline__ int64_t pages_of(int64_t n, int page) { return (n + page - 1) / page; }
 
+// What a block keeps of every request, in shared memory.
+struct StepRequest {
+  int32_t* start;  // [requests + 1] first token
+  int32_t* base;   // [requests] pages given before this request's; -1 refused
+  int32_t* len;    // [requests] tokens cached
+};
+
 // Every block of the one cluster runs the same two prefix sums over the requests (tokens, then
 // pages needed), which costs less than a second launch or a barrier to share them, and then
-// takes its share of the tables' new entries and of the step's tokens.  A token finds its request by
-// bisection of the starts in shared memory; its page is read from the table when the request
-// held it before, else from the free stack, so no block waits for the entries another writes.
-// What the caller may ask for in place (lens, free_count) is written after the cluster barrier
-// that follows the last read.  Bound by latency: launch, two scans, one dependent table load.
+// takes its share of the tables' new entries and of the step's tokens, four a thread: the
+// first one's request by bisection of the starts in shared memory, the others from there.  A
+// token's page is read from the table when the request held it before, else from the free
+// stack, so no block waits for the entries another writes.  What the caller may ask for in
+// place (lens, free_count) is written once every block has read it: the arrival at the cluster
+// barrier stands behind the last read, the wait before the write.  Lengths are below 2^31, so
+// length + tokens and its pages are exact in 32 unsigned bits.
+// Bound by latency: launch, lengths, two scans, a dependent page, the stores.  256 requests with
+// a token each: 5 us of the device's time, of which an empty kernel takes 2.
 __global__ void __launch_bounds__(kStepThreads, 1) plan_step_kernel(const StepArgs a) {
   extern __shared__ int32_t step_smem[];
-  int32_t* start = step_smem;                  // [requests + 1]
-  int32_t* base = step_smem + a.requests + 1;  // pages given before this request's; -1 refused
+  const StepRequest q = {step_smem, step_smem + a.requests + 1, step_smem + 2 * a.requests + 1};
   __shared__ int64_t part[32];
   __shared__ int used;
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const uint32_t page = a.page;
+  const auto pages = [&](uint32_t n) { return n / page + (n % page != 0); };
   if (tid == 0) used = 0;
   const int64_t fc = min(max((int64_t)*a.free_count, (int64_t)0), a.pool);
   int64_t tokens_before = 0, need_before = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += kStepThreads) {
+  for (int r0 = 0; r0 < a.requests; r0 += threads) {
     const int r = r0 + tid;
     const bool live = r < a.requests;
-    const int64_t len = live ? max(a.lens[r], 0) : 0, n = live ? max(a.brings[r], 0) : 0;
+    const uint32_t len = live ? max(a.lens[r], 0) : 0, n = live ? max(a.brings[r], 0) : 0;
     int64_t total;
-    const int64_t through = block_scan_inclusive(n, part, total) + tokens_before;
+    const int64_t through = block_scan_inclusive((int64_t)n, part, total) + tokens_before;
     tokens_before += total;
-    const int64_t held = pages_of(len, a.page), wants = pages_of(len + n, a.page);
-    const bool fits = live && wants <= a.columns && through <= a.tokens;
+    const uint32_t held = pages(len), wants = pages(len + n);
+    const bool fits = live && wants <= (uint32_t)a.columns && through <= a.tokens;
     const int64_t need = fits ? wants - held : 0;
     const int64_t taken = block_scan_inclusive(need, part, total) + need_before;
     need_before += total;
     const bool ok = fits && (need == 0 || taken <= fc);
     if (live) {
-      start[r] = (int32_t)min(through - n, (int64_t)INT32_MAX);
-      base[r] = ok ? (int32_t)(taken - need) : -1;
+      q.start[r] = (int32_t)min(through - n, (int64_t)INT32_MAX);
+      q.base[r] = ok ? (int32_t)(taken - need) : -1;
+      q.len[r] = (int32_t)len;
       if (ok && need > 0) atomicMax(&used, (int)taken);
     }
   }
-  if (tid == 0) start[a.requests] = (int32_t)min(tokens_before, (int64_t)INT32_MAX);
+  if (tid == 0) q.start[a.requests] = (int32_t)min(tokens_before, (int64_t)INT32_MAX);
   __syncthreads();
+  cluster_arrive_release();
 
-  // new table entries, a warp per request
-  const int warps = kStepThreads / 32, lane = tid & 31;
-  for (int r = rank * warps + (tid >> 5); r < a.requests; r += ranks * warps) {
-    const int b = base[r];
+  // new table entries: a thread per request where no block has more than one each, else a warp
+  const bool short_ones = a.requests <= threads;
+  const int lane = short_ones ? 0 : tid & 31, lanes = short_ones ? 1 : 32;
+  const int groups = threads / lanes;
+  for (int r = rank * groups + (short_ones ? tid : tid >> 5); r < a.requests; r += ranks * groups) {
+    const int b = q.base[r];
     if (b < 0) continue;
-    const int64_t len = max(a.lens[r], 0), n = start[r + 1] - start[r];
-    const int held = (int)pages_of(len, a.page), wants = (int)pages_of(len + n, a.page);
-    for (int c = held + lane; c < wants; c += 32)
+    const uint32_t len = q.len[r];
+    const int held = (int)pages(len), wants = (int)pages(len + (uint32_t)(q.start[r + 1] - q.start[r]));
+    for (int c = held + lane; c < wants; c += lanes)
       a.tables[r * a.table_stride + c] = a.free_pages[fc - 1 - (b + c - held)];
   }
-  for (int64_t i = (int64_t)rank * kStepThreads + tid; i < a.tokens;
-       i += (int64_t)ranks * kStepThreads) {
-    int64_t slot = -1;
-    int position = -1;
-    if (i < start[a.requests]) {
-      int lo = 0, hi = a.requests;  // the last request that starts at or before i
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= i) lo = mid;
+  const int tokens_end = q.start[a.requests];
+  for (int64_t i0 = 4 * ((int64_t)rank * threads + tid); i0 < a.tokens;
+       i0 += 4 * (int64_t)ranks * threads) {
+    int64_t slot[4];
+    int32_t position[4];
+    int r = 0;
+    if (i0 < tokens_end) {  // the last request that starts at or before i0
+      int hi = a.requests;
+      while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (q.start[mid] <= i0) r = mid;
         else hi = mid;
       }
-      if (base[lo] >= 0) {
-        const int64_t len = max(a.lens[lo], 0);
-        const int64_t p = len + i - start[lo];
-        const int64_t c = p / a.page, held = pages_of(len, a.page);
-        const int64_t id = c < held ? a.tables[lo * a.table_stride + c]
-                                    : a.free_pages[fc - 1 - (base[lo] + c - held)];
-        slot = id * a.page + (p - c * a.page);
-        position = (int)p;
+    }
+    int at_request = -1;
+    uint32_t at_page = 0;
+    int64_t id = -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = i0 + j;
+      slot[j] = -1;
+      position[j] = -1;
+      if (i >= tokens_end) continue;
+      while (q.start[r + 1] <= i) ++r;
+      if (q.base[r] < 0) continue;
+      const uint32_t len = q.len[r], p = len + (uint32_t)(i - q.start[r]), c = p / page;
+      if (r != at_request || c != at_page) {
+        const uint32_t held = pages(len);
+        id = c < held ? a.tables[r * a.table_stride + c]
+                      : a.free_pages[fc - 1 - (int64_t)(q.base[r] + c - held)];
+        at_request = r;
+        at_page = c;
       }
+      slot[j] = id * page + (p - c * page);
+      position[j] = (int32_t)p;
     }
-    a.slots[i] = slot;
-    a.positions[i] = position;
+    if (i0 + 4 <= a.tokens && (((uintptr_t)a.slots | (uintptr_t)a.positions) & 15) == 0) {
+      reinterpret_cast<longlong2*>(a.slots + i0)[0] = make_longlong2(slot[0], slot[1]);
+      reinterpret_cast<longlong2*>(a.slots + i0)[1] = make_longlong2(slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.positions + i0) =
+          make_int4(position[0], position[1], position[2], position[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j < a.tokens) {
+          a.slots[i0 + j] = slot[j];
+          a.positions[i0 + j] = position[j];
+        }
+    }
   }
-  cluster.sync();
-  if (rank == 0) {
-    for (int r = tid; r <= a.requests; r += kStepThreads) {
-      a.starts[r] = start[r];
-      if (r == a.requests) break;
-      a.granted[r] = base[r] >= 0;
-      const int len = a.lens[r];
-      a.lens_out[r] = base[r] >= 0 ? max(len, 0) + start[r + 1] - start[r] : len;
-    }
-    if (tid == 0) *a.free_count_out = (int32_t)(fc - used);
+  cluster_wait_acquire();
+  for (int r = rank * threads + tid; r < a.requests; r += ranks * threads) {
+    const int n = q.start[r + 1] - q.start[r], len = a.lens[r];
+    a.starts[r] = q.start[r];
+    a.granted[r] = q.base[r] >= 0;
+    a.lens_out[r] = q.base[r] >= 0 ? q.len[r] + n : len;
+  }
+  if (rank == 0 && tid == 0) {
+    a.starts[a.requests] = q.start[a.requests];
+    *a.free_count_out = (int32_t)(fc - used);
   }
 }
 
@@ -174,8 +217,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) release_pages_kernel(const Re
 
 // One launch of a single cluster of `blocks`.
 template <typename Args>
-static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, size_t smem,
-                          void* stream, const char* what) {
+static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, int threads,
+                          size_t smem, void* stream, const char* what) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -186,7 +229,7 @@ static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, si
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kStepThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr = {};
@@ -343,11 +386,14 @@ extern "C" int tr_plan_step(const int32_t* lens, const int32_t* new_tokens, int6
   StepArgs a = {lens, new_tokens, tables, table_stride, free_pages, free_count, slots, positions,
                 starts, lens_out, granted, free_count_out, pool, tokens, (int)requests, columns,
                 page_size};
-  // one block serves a decode step; the cluster of 8 pays its barrier back from a few tokens
-  // per thread on
-  const int blocks = tokens + requests > 4 * kStepThreads ? 8 : 1;
-  return launch_cluster(plan_step_kernel, a, blocks, (2 * requests + 1) * sizeof(int32_t), stream,
-                        "tr_plan_step");
+  // one block serves a decode step, of as many threads as it has requests or groups of four
+  // tokens (barriers of fewer warps are cheaper); the cluster of 8 pays its barrier back from a
+  // few tokens per thread on
+  const int64_t work = std::max(requests, tokens / 4);
+  const int blocks = tokens > 8 * kStepThreads ? 8 : 1;
+  const int threads = blocks > 1 || work > 512 ? kStepThreads : work > 256 ? 512 : 256;
+  return launch_cluster(plan_step_kernel, a, blocks, threads, (3 * requests + 1) * sizeof(int32_t),
+                        stream, "tr_plan_step");
 }
 
 extern "C" int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t requests,
@@ -360,8 +406,8 @@ extern "C" int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t 
   ReleaseArgs a = {lens, finished, tables, table_stride, free_pages, free_count, pool,
                    (int)requests, columns, page_size};
   const int blocks = requests * columns > 4 * kStepThreads ? 8 : 1;
-  return launch_cluster(release_pages_kernel, a, blocks, requests * sizeof(int32_t), stream,
-                        "tr_release_pages");
+  return launch_cluster(release_pages_kernel, a, blocks, kStepThreads, requests * sizeof(int32_t),
+                        stream, "tr_release_pages");
 }
 
 extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride,

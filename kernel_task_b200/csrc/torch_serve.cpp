@@ -77,7 +77,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   if (page_size < 1 || page_size > INT32_MAX) refuse(op, "page_size must be positive");
   if (tokens < 0) refuse(op, "tokens must not be negative");
   if (tables.size(1) > INT32_MAX) refuse(op, "too many table columns");
-  c10::cuda::CUDAGuard guard(lens.device());
+  const c10::cuda::CUDAGuard guard(lens.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
   const auto ints = lens.options();
   at::Tensor slots = at::empty({tokens}, ints.dtype(at::kLong));
   at::Tensor positions = at::empty({tokens}, ints), starts = at::empty({R + 1}, ints),
@@ -110,7 +111,8 @@ void release_pages(const at::Tensor& lens, const at::Tensor& finished, const at:
   need_vector(op, "free_count", free_count, at::kInt, 1, lens);
   if (page_size < 1 || page_size > INT32_MAX) refuse(op, "page_size must be positive");
   if (tables.size(1) > INT32_MAX) refuse(op, "too many table columns");
-  c10::cuda::CUDAGuard guard(lens.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
+  const c10::cuda::CUDAGuard guard(lens.device());
   check(tr_release_pages(lens.data_ptr<int32_t>(), finished.data_ptr<int32_t>(), R,
                          tables.data_ptr<int32_t>(), row_stride(tables), (int32_t)tables.size(1),
                          free_pages.data_ptr<int32_t>(), free_pages.size(0),
@@ -147,7 +149,8 @@ void append_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pag
     refuse(op, "k and v must be [tokens, " + std::to_string(k_pages.size(1)) + ", " +
                    std::to_string(k_pages.size(3)) + "]");
   need_vector(op, "slots", slots, at::kLong, k.size(0), k);
-  c10::cuda::CUDAGuard guard(k.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
+  const c10::cuda::CUDAGuard guard(k.device());
   const at::Tensor kc = k.stride(2) == 1 || k.size(2) == 1 ? k : k.contiguous();
   const at::Tensor vc = v.stride(2) == 1 || v.size(2) == 1 ? v : v.contiguous();
   check(tr_append_kv(kc.data_ptr(), kc.stride(0), kc.stride(1), vc.data_ptr(), vc.stride(0),
@@ -226,7 +229,8 @@ std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::
   if (H > INT32_MAX || tables.size(1) > INT32_MAX) refuse(op, "shape too large");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
   if (!(s > 0) || !std::isfinite((float)s)) refuse(op, "scale must be positive and finite");
-  c10::cuda::CUDAGuard guard(q.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
+  const c10::cuda::CUDAGuard guard(q.device());
   // heads of the last axis contiguous and 16-byte aligned, or a copy that is
   const int64_t es = q.element_size();
   const bool fine = q.stride(2) == 1 && ((uintptr_t)q.data_ptr() & 15) == 0 &&
@@ -308,7 +312,8 @@ std::pair<OptTensor, OptTensor> residual_norm(const OptTensor& y, const at::Tens
                      "]");
     return W > 1 && t.stride(1) != 1 ? t.contiguous() : t;
   };
-  c10::cuda::CUDAGuard guard(h.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
+  const c10::cuda::CUDAGuard guard(h.device());
   at::Tensor hc = rows("h", h), yc, gc;
   n.h = hc.data_ptr();
   n.h_stride = row_stride(hc);
@@ -369,7 +374,8 @@ std::pair<at::Tensor, at::Tensor> sample_tokens(const at::Tensor& logits, const 
   if (top_k.has_value()) need_vector(op, "top_k", *top_k, at::kInt, R, logits);
   if (top_p.has_value()) need_vector(op, "top_p", *top_p, at::kFloat, R, logits);
   if (min_p.has_value()) need_vector(op, "min_p", *min_p, at::kFloat, R, logits);
-  c10::cuda::CUDAGuard guard(logits.device());
+  const at::AutoDispatchBelowADInplaceOrView no_grad;
+  const c10::cuda::CUDAGuard guard(logits.device());
   const at::Tensor lc = V > 1 && logits.stride(1) != 1 ? logits.contiguous() : logits;
   const at::Tensor nc = V > 1 && noise.stride(1) != 1 ? noise.contiguous() : noise;
   at::Tensor tokens = at::empty({R}, logits.options().dtype(at::kLong));
