@@ -8,6 +8,16 @@ torch.compile, CUDA graphs and other custom-op machinery:
     g = torch.ops.trring.accumulate(x, handle)               # fn.accumulate(x), fp32
     torch.ops.trring.consume_silu_mul(g, u), torch.ops.trring.consume_add(h, y)
 
+and the serving operators (serve.py), with positional arguments:
+
+    slots, positions, starts, lens, granted, free_count = torch.ops.trring.plan_step(
+        lens, new, tables, free, free_count, page_size, tokens)
+    torch.ops.trring.append_kv(k, v, k_pages, v_pages, slots)
+    out, lse = torch.ops.trring.paged_attention(q, k_pages, v_pages, tables, lens, starts, scale)
+    h, x = torch.ops.trring.residual_norm(y, h, post, pre, gate, post_bias, pre_bias, kind, eps,
+                                          residual_scale, branch_scale)
+    ids, logprobs = torch.ops.trring.sample_tokens(logits, noise, temperature, top_k, top_p, min_p)
+
 A prepared operator is a C++ object, which a custom op cannot take as an argument, so operators
 are registered in a process-local table and the op takes the integer handle.  Each op has a
 fake (meta) implementation giving the output shape and dtype without running a kernel.
@@ -16,9 +26,11 @@ from __future__ import annotations
 
 import itertools
 import threading
+from typing import Optional
 
 import torch
 
+from . import serve as _serve
 from .ring import consume_add as _consume_add
 from .ring import consume_silu_mul as _consume_silu_mul
 from .spec import TRSpec
@@ -117,3 +129,71 @@ def consume_add(h: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
 @consume_add.register_fake
 def _(h, y):
     return torch.empty_like(h)
+
+
+@torch.library.custom_op("trring::plan_step", mutates_args=("tables",))
+def plan_step(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torch.Tensor,
+              free_count: torch.Tensor, page_size: int, tokens: int) -> tuple[
+                  torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                  torch.Tensor]:
+    return tuple(_serve.plan_step(lens, new, tables, free, free_count, page_size, tokens))
+
+
+@plan_step.register_fake
+def _(lens, new, tables, free, free_count, page_size, tokens):
+    R = lens.shape[0]
+    return (lens.new_empty(tokens, dtype=torch.int64), lens.new_empty(tokens),
+            lens.new_empty(R + 1), lens.new_empty(R), lens.new_empty(R), lens.new_empty(1))
+
+
+@torch.library.custom_op("trring::append_kv", mutates_args=("k_pages", "v_pages"))
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+              slots: torch.Tensor) -> None:
+    _serve.append_kv(k, v, k_pages, v_pages, slots)
+
+
+@append_kv.register_fake
+def _(k, v, k_pages, v_pages, slots):
+    return None
+
+
+@torch.library.custom_op("trring::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    tables: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                    scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    return _serve.paged_attention(q, k_pages, v_pages, tables, lens, starts, scale=scale,
+                                  return_lse=True)
+
+
+@paged_attention.register_fake
+def _(q, k_pages, v_pages, tables, lens, starts, scale=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.custom_op("trring::residual_norm", mutates_args=())
+def residual_norm(y: torch.Tensor, h: torch.Tensor, post: Optional[torch.Tensor],
+                  pre: torch.Tensor, gate: Optional[torch.Tensor],
+                  post_bias: Optional[torch.Tensor], pre_bias: Optional[torch.Tensor], kind: str,
+                  eps: float, residual_scale: float,
+                  branch_scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return _serve.residual_norm(y, h, post=post, pre=pre, gate=gate, post_bias=post_bias,
+                                pre_bias=pre_bias, kind=kind, eps=eps,
+                                residual_scale=residual_scale, branch_scale=branch_scale)
+
+
+@residual_norm.register_fake
+def _(y, h, post, pre, gate, post_bias, pre_bias, kind, eps, residual_scale, branch_scale):
+    return h.new_empty(h.shape), h.new_empty(h.shape)
+
+
+@torch.library.custom_op("trring::sample_tokens", mutates_args=())
+def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor,
+                  top_k: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
+                  min_p: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    return _serve.sample_tokens(logits, noise, temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@sample_tokens.register_fake
+def _(logits, noise, temperature, top_k, top_p, min_p):
+    R = logits.shape[0]
+    return (logits.new_empty(R, dtype=torch.int64), logits.new_empty(R, dtype=torch.float32))
