@@ -13,6 +13,8 @@
 // Split.  An item is (request, row tile, kv head), a unit one block of keys of an item.  The
 // blocks of the grid take equal contiguous runs of all units, found by one prefix sum over the
 // requests, so ragged lengths balance to within a block of keys without the host knowing them.
+// Each warp's loads run two blocks ahead along the run, over the ends of items too: with short
+// contexts an item is over in the time of one memory access.
 // An item that several blocks share leaves fp32 partial results in the workspace; the last block
 // to arrive joins them in unit order, so the result does not depend on the order of arrival.
 #include <algorithm>
@@ -24,8 +26,11 @@ namespace trr {
 
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = 32 * kRowsWarps;
-constexpr int kRowsStages = 3;
-constexpr int kMinBlocks = 2;  // blocks of keys a grid block takes at least
+// stages of a warp: three, or two for tiles of 16 rows, whose exchange buffer takes the third's room
+template <int NT>
+__host__ __device__ constexpr int rows_stages() {
+  return NT == 1 ? 3 : 2;
+}
 
 // 16 keys of 128 elements or 32 of 64: 8 KB of keys and values a warp and stage
 template <int D>
@@ -55,102 +60,189 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-struct RowsWork {
-  int64_t units;       // of all requests
-  int64_t request_u0;  // first unit of `request`
-  int64_t request_i0;  // first item of `request`
-  int request;         // the request of this block's first unit
-};
-
-struct RequestShape {
-  int n, tiles, blocks;
-  int64_t items, units;
+// Walks the items of a contiguous run of units.
+struct RowsItem {
+  int request, rows, tiles, tile, kvh;
+  int blocks;      // units of the item: blocks of keys, at least one (rows without keys are written too)
+  int see0, cap;   // token i of the request sees min(see0 + i, cap) keys (none if negative)
+  int64_t token0;  // the request's first token
+  int64_t u0;      // first unit of the item
+  int64_t index;   // item number
 };
 template <int ROWS, int BK>
-__device__ __forceinline__ RequestShape shape_of(const tr_attention& a, int r) {
-  RequestShape s;
-  s.n = brought(a, r);
-  s.tiles = (int)(((int64_t)s.n * (a.heads / a.kv_heads) + ROWS - 1) / ROWS);
-  s.blocks = max((cached(a, r) + BK - 1) / BK, 1);  // at least one: rows without keys are written too
-  s.items = (int64_t)s.tiles * a.kv_heads;
-  s.units = s.items * s.blocks;
-  return s;
+__device__ __forceinline__ void open_request(const tr_attention& a, int g, RowsItem& it, int r) {
+  const int n = brought(a, r);
+  it.request = r;
+  it.rows = n * g;
+  it.tiles = (it.rows + ROWS - 1) / ROWS;
+  it.tile = it.kvh = 0;
+  it.cap = cached(a, r);
+  it.blocks = max((it.cap + BK - 1) / BK, 1);
+  it.see0 = (int)max((int64_t)a.lens[r] - n + 1, -(int64_t)(1 << 30));
+  it.token0 = max((int64_t)a.starts[r], (int64_t)0);
+}
+template <int ROWS, int BK>
+__device__ __forceinline__ void next_item(const tr_attention& a, int g, RowsItem& it) {
+  it.u0 += it.blocks;
+  ++it.index;
+  if (++it.kvh < a.kv_heads) return;
+  it.kvh = 0;
+  if (++it.tile < it.tiles) return;
+  while (it.request + 1 < (int)a.requests) {
+    open_request<ROWS, BK>(a, g, it, it.request + 1);
+    if (it.tiles) return;
+  }
+}
+__device__ __forceinline__ int keys_of_row(const RowsItem& it, int g, int row) {
+  return max(min(it.see0 + row / g, it.cap), 0);
+}
+
+// The run of units of this block, and the item it starts in; false when there is none.  Up to 32
+// requests every warp sums them by itself, else thread i takes requests [i per, (i + 1) per).
+template <int ROWS, int BK>
+__device__ __forceinline__ bool find_run(const tr_attention& a, int g, int64_t max_items,
+                                         int64_t (&part)[2][32], RowsItem& first, int64_t& U,
+                                         int64_t& G, int64_t& u_begin, int64_t& u_end) {
+  const int R = (int)a.requests, lane = threadIdx.x & 31;
+  const bool few = R <= 32;
+  const int workers = few ? 32 : (int)blockDim.x, me = few ? lane : (int)threadIdx.x;
+  const int per = (R + workers - 1) / workers;
+  const int r_lo = min(me * per, R), r_hi = min(r_lo + per, R);
+  RowsItem it;
+  int64_t my_units = 0, my_items = 0;
+  for (int r = r_lo; r < r_hi; ++r) {
+    open_request<ROWS, BK>(a, g, it, r);
+    my_items += (int64_t)it.tiles * a.kv_heads;
+    my_units += (int64_t)it.tiles * a.kv_heads * it.blocks;
+  }
+  int64_t through, items_through, items;
+  if (few) {
+    through = warp_scan_inclusive(my_units);
+    items_through = warp_scan_inclusive(my_items);
+    U = __shfl_sync(0xffffffffu, through, 31);
+    items = __shfl_sync(0xffffffffu, items_through, 31);
+  } else {
+    through = block_scan_inclusive(my_units, part[0], U);
+    items_through = block_scan_inclusive(my_items, part[1], items);
+  }
+  if (U == 0 || items > max_items) return false;
+  // Blocks to share the units: a part of an item costs the block that joins it about a third of
+  // a block of keys, so an item of b blocks is best cut into sqrt(3 b) parts (one request of
+  // 32768 keys over one kv head: 60 us, 77 us on all blocks of the grid)
+  G = min(min((int64_t)gridDim.x, U), (int64_t)ceilf(sqrtf(3.f * (float)U * (float)items)));
+  if (blockIdx.x >= G) return false;
+  u_begin = U * blockIdx.x / G;
+  u_end = U * (blockIdx.x + 1) / G;
+  const bool mine = through - my_units <= u_begin && u_begin < through;
+  int64_t u0 = through - my_units, index = items_through - my_items;
+  int request = r_lo;
+  if (mine) {
+    for (; request < r_hi; ++request) {
+      open_request<ROWS, BK>(a, g, it, request);
+      const int64_t units = (int64_t)it.tiles * a.kv_heads * it.blocks;
+      if (u_begin < u0 + units) break;
+      u0 += units;
+      index += (int64_t)it.tiles * a.kv_heads;
+    }
+  }
+  if (few) {
+    const int who = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+    request = __shfl_sync(0xffffffffu, request, who);
+    u0 = __shfl_sync(0xffffffffu, u0, who);
+    index = __shfl_sync(0xffffffffu, index, who);
+  } else {
+    if (mine) part[0][0] = u0, part[0][1] = index, part[0][2] = request;
+    __syncthreads();
+    u0 = part[0][0], index = part[0][1], request = (int)part[0][2];
+  }
+  open_request<ROWS, BK>(a, g, first, request);
+  const int item = (int)((u_begin - u0) / first.blocks);
+  first.u0 = u0 + (int64_t)item * first.blocks;
+  first.index = index + item;
+  first.tile = item / a.kv_heads;
+  first.kvh = item - first.tile * a.kv_heads;
+  return true;
 }
 
 template <typename E, int D, int NT>
-__global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_attention a, int* counters,
-                                                                  int64_t max_items,
-                                                                  float* partials) {
+__global__ void __launch_bounds__(kRowsThreads, 2) attend_rows_kernel(const tr_attention a,
+                                                                     int* counters,
+                                                                     int64_t max_items,
+                                                                     float* partials) {
   constexpr int ROWS = 8 * NT, WK = warp_keys<D>(), MT = WK / 16, BK = block_keys<D>();
-  constexpr int CPR = D / 8;                      // 16-byte chunks of a row
-  constexpr int STAGE = 2 * WK * D * 2;           // bytes of a warp's stage: keys, then values
-  constexpr int PAD = D + 4;                      // row stride of the joined outputs
+  constexpr int STAGES = rows_stages<NT>();
+  constexpr int CPR = D / 8;                // 16-byte chunks of a row
+  constexpr int STAGE = 2 * WK * D * 2;     // bytes of a warp's stage: keys, then values
+  constexpr int F = D / 16 / kRowsWarps;    // 16-element slices of the output that a warp ends with
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int64_t scan_part[32], scan_items[32];
-  __shared__ RowsWork work;
+  __shared__ int64_t part[2][32];
   __shared__ float sh_m[kRowsWarps][ROWS], sh_l[kRowsWarps][ROWS];
   __shared__ int sh_last;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.heads / a.kv_heads;
-  const int R = (int)a.requests;
   clear_outside<E>(a, (int64_t)blockIdx.x * kRowsThreads + tid, (int64_t)gridDim.x * kRowsThreads);
-  if (R == 0) return;
+  if (a.requests == 0) return;
+  RowsItem it;
+  int64_t U, G, u_begin, u_end;
+  if (!find_run<ROWS, BK>(a, g, max_items, part, it, U, G, u_begin, u_end)) return;
 
-  // ---- this block's run of units: thread i sums requests [i per, (i + 1) per)
-  const int per = (R + kRowsThreads - 1) / kRowsThreads;
-  const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
-  int64_t my_units = 0, my_items = 0;
-  for (int r = r_lo; r < r_hi; ++r) {
-    const RequestShape s = shape_of<ROWS, BK>(a, r);
-    my_units += s.units;
-    my_items += s.items;
-  }
-  int64_t U, all_items;
-  const int64_t through = block_scan_inclusive(my_units, scan_part, U);
-  const int64_t items_through = block_scan_inclusive(my_items, scan_items, all_items);
-  if (U == 0 || all_items > max_items) return;
-  const int64_t G = min((int64_t)gridDim.x, (U + kMinBlocks - 1) / kMinBlocks);
-  if (blockIdx.x >= G) return;
-  const int64_t u_begin = U * blockIdx.x / G, u_end = U * (blockIdx.x + 1) / G;
-  if (through - my_units <= u_begin && u_begin < through) {
-    int64_t u = through - my_units, it = items_through - my_items;
-    int r = r_lo;
-    for (; r < r_hi; ++r) {
-      const RequestShape s = shape_of<ROWS, BK>(a, r);
-      if (u_begin < u + s.units) break;
-      u += s.units;
-      it += s.items;
-    }
-    work.request = r;
-    work.request_u0 = u;
-    work.request_i0 = it;
-  }
-  __syncthreads();
-  int request = work.request;
-  int64_t request_u0 = work.request_u0, request_i0 = work.request_i0;
-  RequestShape shape = shape_of<ROWS, BK>(a, request);
-
-  const uint32_t stage0 = smem_u32(smem) + warp * kRowsStages * STAGE;
-  const E* kp = static_cast<const E*>(a.k_pages);
-  const E* vp = static_cast<const E*>(a.v_pages);
+  const uint32_t stage0 = smem_u32(smem) + warp * STAGES * STAGE;
+  float4* exchange = reinterpret_cast<float4*>(smem + kRowsWarps * STAGES * STAGE);
+  const uint4* kp = static_cast<const uint4*>(a.k_pages);
+  const uint4* vp = static_cast<const uint4*>(a.v_pages);
   const float scale2 = a.scale * kLog2e;
   const int page_shift = 31 - __clz(a.page_size);
 
-  for (int64_t u = u_begin; u < u_end;) {
-    while (u >= request_u0 + shape.units) {
-      request_u0 += shape.units;
-      request_i0 += shape.items;
-      shape = shape_of<ROWS, BK>(a, ++request);
+  // ---- loads.  `ahead` is the item of unit `lu`, the next to load; `rows_next` the pool rows of
+  // its keys (lane i < WK: the warp's key i), ~0u past the keys and for bad pages
+  RowsItem ahead = it;
+  int64_t lu = u_begin;
+  uint32_t rows_next = ~0u;
+  int keys_ahead = 0;
+  const auto open_ahead = [&] {
+    keys_ahead = keys_of_row(ahead, g, min((ahead.tile + 1) * ROWS, ahead.rows) - 1);
+  };
+  const auto find_rows = [&] {
+    const int key = (int)(lu - ahead.u0) * BK + warp * WK + lane;
+    rows_next = ~0u;
+    if (lu < u_end && lane < WK && key < keys_ahead) {
+      const int id = a.tables[ahead.request * a.table_stride + (key >> page_shift)];
+      if (id >= 0 && id < a.pages)
+        rows_next = (uint32_t)((id * (int64_t)a.kv_heads + ahead.kvh) * a.page_size +
+                               (key & (a.page_size - 1)));
     }
-    const int64_t in_request = u - request_u0;
-    const int item = (int)(in_request / shape.blocks);
-    const int b_first = (int)(in_request - (int64_t)item * shape.blocks);
-    const int b_last = (int)min((int64_t)shape.blocks, b_first + (u_end - u));  // one past
-    const int64_t item_u0 = request_u0 + (int64_t)item * shape.blocks;
-    const int tile = item / a.kv_heads, kvh = item - tile * a.kv_heads;
-    const int rows_here = min((int64_t)ROWS, (int64_t)shape.n * g - (int64_t)tile * ROWS);
-    const int64_t token0 = max(a.starts[request], 0);
+  };
+  const auto load = [&] {  // one commit group, empty past the run
+    if (lu < u_end) {
+      const uint32_t base = stage0 + (uint32_t)(lu - u_begin) % STAGES * STAGE;
+#pragma unroll
+      for (int i = 0; i < WK * CPR / 32; ++i) {
+        const int row = i * (32 / CPR) + lane / CPR, c = lane % CPR;
+        const uint32_t r = __shfl_sync(0xffffffffu, rows_next, row);
+        const bool held = r != ~0u;
+        const uint64_t at = (uint64_t)(held ? r : 0u) * CPR + c;
+        const uint32_t dst = base + row * (D * 2) + ((c ^ (row & 7)) << 4);
+        copy16_async(dst, kp + at, held);
+        copy16_async(dst + WK * D * 2, vp + at, held);
+      }
+      if (++lu == ahead.u0 + ahead.blocks && lu < u_end) {
+        next_item<ROWS, BK>(a, g, ahead);
+        open_ahead();
+      }
+      find_rows();
+    }
+    copies_commit();
+  };
+  open_ahead();
+  find_rows();
+#pragma unroll 1
+  for (int s = 0; s < STAGES - 1; ++s) load();
+
+  for (int64_t u = u_begin; u < u_end; next_item<ROWS, BK>(a, g, it)) {
+    const int b_first = (int)(u - it.u0);
+    const int b_last = (int)min((int64_t)it.blocks, b_first + (u_end - u));  // one past
+    const int rows_here = min(ROWS, it.rows - it.tile * ROWS);
 
     // the two query rows of this lane's columns, per n-tile: how many keys they see
     int limit[NT][2];
@@ -159,20 +251,16 @@ __global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_atte
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = nt * 8 + (lane & 3) * 2 + e;
-        limit[nt][e] =
-            row < rows_here ? visible(a, request, shape.n, (tile * ROWS + row) / g) : 0;
+        limit[nt][e] = row < rows_here ? keys_of_row(it, g, it.tile * ROWS + row) : 0;
       }
-    const int keys_end =
-        max(visible(a, request, shape.n, (tile * ROWS + rows_here - 1) / g), 0);
-    const int b_stop = min(b_last, (keys_end + BK - 1) / BK);
 
     // Q^T fragments: row lane / 4, elements ks * 16 + (lane & 3) * 2 (+1, +8, +9)
     uint32_t qf[NT][D / 16][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = nt * 8 + (lane >> 2), at = tile * ROWS + row;
-      const int i = at / g, h = kvh * g + (at - i * g);
-      const E* q = static_cast<const E*>(a.q) + (token0 + i) * a.q_token_stride +
+      const int row = nt * 8 + (lane >> 2), at = it.tile * ROWS + row;
+      const int i = at / g, h = it.kvh * g + (at - i * g);
+      const E* q = static_cast<const E*>(a.q) + (it.token0 + i) * a.q_token_stride +
                    h * a.q_head_stride + (lane & 3) * 2;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
@@ -193,46 +281,11 @@ __global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_atte
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
     }
 
-    const int32_t* table = a.tables + request * a.table_stride;
-    // lane i < WK: page of key i of the warp's share of block b (-1 past the end)
-    const auto page_id = [&](int b) {
-      const int key = b * BK + warp * WK + lane;
-      return lane < WK && b < b_stop && key < keys_end ? table[key >> page_shift] : -1;
-    };
-    const auto load = [&](int b, int id) {  // one commit group, empty past the end
-      if (b < b_stop) {
-        const uint32_t base = stage0 + (b - b_first) % kRowsStages * STAGE;
-        const int key0 = b * BK + warp * WK;
-#pragma unroll
-        for (int i = 0; i < WK * CPR / 32; ++i) {
-          const int row = i * (32 / CPR) + lane / CPR, c = lane % CPR, key = key0 + row;
-          const int pid = __shfl_sync(0xffffffffu, id, row);
-          const bool held = pid >= 0 && pid < a.pages && key < keys_end;
-          const int64_t at =
-              held ? (((int64_t)pid * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1))) *
-                             D + c * 8
-                   : 0;
-          const uint32_t dst = base + row * (D * 2) + ((c ^ (row & 7)) << 4);
-          copy16_async(dst, kp + at, held);
-          copy16_async(dst + WK * D * 2, vp + at, held);
-        }
-      }
-      copies_commit();
-    };
-    int ids = page_id(b_first);
-    for (int s = 0; s < kRowsStages - 1; ++s) {
-      const int next = page_id(b_first + s + 1);
-      load(b_first + s, ids);
-      ids = next;
-    }
-
-    for (int b = b_first; b < b_stop; ++b) {
-      const int next = page_id(b + kRowsStages);
-      load(b + kRowsStages - 1, ids);
-      ids = next;
-      copies_wait<kRowsStages - 1>();
+    for (int b = b_first; b < b_last; ++b, ++u) {
+      load();
+      copies_wait<STAGES - 1>();
       __syncwarp();
-      const uint32_t ks0 = stage0 + (b - b_first) % kRowsStages * STAGE, vs0 = ks0 + WK * D * 2;
+      const uint32_t ks0 = stage0 + (uint32_t)(u - u_begin) % STAGES * STAGE, vs0 = ks0 + WK * D * 2;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float s[NT][4];
@@ -295,13 +348,11 @@ __global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_atte
           for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][i], vf, pf[nt][0], pf[nt][1], E());
         }
       }
-      __syncwarp();  // the stage is read before the next load overwrites it
+      __syncwarp();  // the stage is read before a later load overwrites it
     }
-    copies_wait<0>();
-    __syncthreads();
 
-    // ---- join the four warps
-    float* so = reinterpret_cast<float*>(smem);  // [warp][row][PAD]
+    // ---- join the four warps: warp w ends with slices w F .. w F + F - 1 of the output, as
+    // fragments of 16 elements by 8 rows; the other slices go to their warps
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -312,111 +363,174 @@ __global__ void __launch_bounds__(kRowsThreads) attend_rows_kernel(const tr_atte
         v += __shfl_xor_sync(0xffffffffu, v, 16);
         const int row = nt * 8 + (lane & 3) * 2 + e;
         if (lane < 4) sh_m[warp][row] = m[nt][e], sh_l[warp][row] = v;
+      }
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          so[(warp * ROWS + row) * PAD + i * 16 + (lane >> 2)] = o[nt][i][e];
-          so[(warp * ROWS + row) * PAD + i * 16 + (lane >> 2) + 8] = o[nt][i][e + 2];
-        }
+      for (int i = 0; i < D / 16; ++i) {
+        const int to = i / F, from = (warp - to - 1) & 3;  // 0 .. 2 among the others
+        if (to != warp)
+          exchange[(((to * 3 + from) * NT + nt) * F + i % F) * 32 + lane] =
+              make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
       }
     }
     __syncthreads();
-    constexpr int COLS = ROWS * D / kRowsThreads;  // consecutive outputs of a thread
-    const int orow = tid * COLS / D, ocol = tid * COLS % D;
-    float top = -INFINITY, sum = 0.f, acc[COLS];
+    float top[NT][2], sum[NT][2];
+    float4 acc[NT][F];
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[kRowsWarps][2];
 #pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, sh_m[w][orow]);
-    const float base = top == -INFINITY ? 0.f : top;
+      for (int e = 0; e < 2; ++e) {
+        const int row = nt * 8 + (lane & 3) * 2 + e;
+        float t = sh_m[0][row];
 #pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) {
-      const float f = exp2_approx(sh_m[w][orow] - base);
-      sum += f * sh_l[w][orow];
+        for (int w = 1; w < kRowsWarps; ++w) t = fmaxf(t, sh_m[w][row]);
+        const float base = t == -INFINITY ? 0.f : t;
+        top[nt][e] = t;
+        sum[nt][e] = 0.f;
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) acc[c] += f * so[(w * ROWS + orow) * PAD + ocol + c];
+        for (int w = 0; w < kRowsWarps; ++w) {
+          f[w][e] = exp2_approx(sh_m[w][row] - base);
+          sum[nt][e] += f[w][e] * sh_l[w][row];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < F; ++k) {
+        acc[nt][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) {  // in warp order, whoever adds
+          float4 v;
+          if (w == warp) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              if (i == warp * F + k) v = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+          } else {
+            v = exchange[(((warp * 3 + ((w - warp - 1) & 3)) * NT + nt) * F + k) * 32 + lane];
+          }
+          acc[nt][k].x += f[w][0] * v.x, acc[nt][k].y += f[w][1] * v.y;
+          acc[nt][k].z += f[w][0] * v.z, acc[nt][k].w += f[w][1] * v.w;
+        }
+      }
     }
 
     bool writes = true;
-    if (b_last - b_first < shape.blocks) {
+    if (b_last - b_first < it.blocks) {
       // shared with other blocks: leave the partial result, and the last to arrive joins all
-      const int64_t first_block = ((item_u0 + 1) * G - 1) / U;
-      const int64_t last_block = ((item_u0 + shape.blocks) * G - 1) / U;
+      const int64_t first_block = ((it.u0 + 1) * G - 1) / U;
+      const int64_t last_block = ((it.u0 + it.blocks) * G - 1) / U;
       const auto slot = [&](int64_t c) {  // a block's first segment, else its last
-        return partials + (2 * c + (U * c / G < item_u0 ? 1 : 0)) * partial_floats(ROWS, D);
+        return partials + (2 * c + (U * c / G < it.u0 ? 1 : 0)) * partial_floats(ROWS, D);
       };
+      const auto place = [&](int nt, int k) { return ((warp * NT + nt) * F + k) * 32 + lane; };
       float* mine = slot(blockIdx.x);
 #pragma unroll
-      for (int c = 0; c < COLS; c += 4)
-        __stcg(reinterpret_cast<float4*>(mine + orow * D + ocol + c),
-               make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
-      if (ocol == 0) {
-        __stcg(mine + ROWS * D + orow, top);
-        __stcg(mine + ROWS * D + ROWS + orow, sum);
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int k = 0; k < F; ++k) __stcg(reinterpret_cast<float4*>(mine) + place(nt, k), acc[nt][k]);
+        if (warp == 0 && lane < 4) {
+          float2* ml = reinterpret_cast<float2*>(mine + ROWS * D) + nt * 4 + lane;
+          __stcg(ml, make_float2(top[nt][0], top[nt][1]));
+          __stcg(ml + ROWS / 2, make_float2(sum[nt][0], sum[nt][1]));
+        }
       }
       __syncthreads();
-      const int64_t counter = request_i0 + item;
       if (tid == 0) {
-        const int arrived = atom_add_acq_rel_gpu(counters + counter, 1);
+        const int arrived = atom_add_acq_rel_gpu(counters + it.index, 1);
         sh_last = arrived == (int)(last_block - first_block);
-        if (sh_last) counters[counter] = 0;
+        if (sh_last) counters[it.index] = 0;
       }
       __syncthreads();
       writes = sh_last;
       if (writes) {
-        // eight partial results at a time: their loads are in flight together
-        top = -INFINITY;
-        sum = 0.f;
+        constexpr int AT_ONCE = NT == 1 ? 8 : 4;  // partial results whose loads are in flight together
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
-        for (int64_t c0 = first_block; c0 <= last_block; c0 += 8) {
-          float pm[8], pl[8];
-          float4 pv[8][COLS / 4];
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int e = 0; e < 2; ++e) top[nt][e] = -INFINITY, sum[nt][e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < F; ++k) acc[nt][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        for (int64_t c0 = first_block; c0 <= last_block; c0 += AT_ONCE) {
+          float2 pm[AT_ONCE][NT], pl[AT_ONCE][NT];
+          float4 pv[AT_ONCE][NT][F];
+#pragma unroll
+          for (int j = 0; j < AT_ONCE; ++j) {
             const float* p = slot(min(c0 + j, last_block));
-            pm[j] = c0 + j <= last_block ? __ldcg(p + ROWS * D + orow) : -INFINITY;
-            pl[j] = __ldcg(p + ROWS * D + ROWS + orow);
 #pragma unroll
-            for (int k = 0; k < COLS / 4; ++k)
-              pv[j][k] = __ldcg(reinterpret_cast<const float4*>(p + orow * D + ocol) + k);
+            for (int nt = 0; nt < NT; ++nt) {
+              const float2* ml = reinterpret_cast<const float2*>(p + ROWS * D) + nt * 4 + (lane & 3);
+              pm[j][nt] = c0 + j <= last_block ? __ldcg(ml) : make_float2(-INFINITY, -INFINITY);
+              pl[j][nt] = __ldcg(ml + ROWS / 2);
+#pragma unroll
+              for (int k = 0; k < F; ++k)
+                pv[j][nt][k] = __ldcg(reinterpret_cast<const float4*>(p) + place(nt, k));
+            }
           }
-          float all = top;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) all = fmaxf(all, pm[j]);
-          const float base = all == -INFINITY ? 0.f : all;
-          const float keep = exp2_approx(top - base);
-          top = all;
-          sum *= keep;
+          for (int nt = 0; nt < NT; ++nt) {
+            float base[2], keep[2];
 #pragma unroll
-          for (int c = 0; c < COLS; ++c) acc[c] *= keep;
+            for (int e = 0; e < 2; ++e) {
+              float t = top[nt][e];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float f = exp2_approx(pm[j] - base);
-            sum += f * pl[j];
+              for (int j = 0; j < AT_ONCE; ++j) t = fmaxf(t, e ? pm[j][nt].y : pm[j][nt].x);
+              base[e] = t == -INFINITY ? 0.f : t;
+              keep[e] = exp2_approx(top[nt][e] - base[e]);
+              top[nt][e] = t;
+              sum[nt][e] *= keep[e];
+            }
 #pragma unroll
-            for (int k = 0; k < COLS / 4; ++k) {
-              acc[4 * k] += f * pv[j][k].x, acc[4 * k + 1] += f * pv[j][k].y;
-              acc[4 * k + 2] += f * pv[j][k].z, acc[4 * k + 3] += f * pv[j][k].w;
+            for (int k = 0; k < F; ++k) {
+              acc[nt][k].x *= keep[0], acc[nt][k].y *= keep[1];
+              acc[nt][k].z *= keep[0], acc[nt][k].w *= keep[1];
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+              const float f0 = exp2_approx(pm[j][nt].x - base[0]), f1 = exp2_approx(pm[j][nt].y - base[1]);
+              sum[nt][0] += f0 * pl[j][nt].x;
+              sum[nt][1] += f1 * pl[j][nt].y;
+#pragma unroll
+              for (int k = 0; k < F; ++k) {
+                acc[nt][k].x += f0 * pv[j][nt][k].x, acc[nt][k].y += f1 * pv[j][nt][k].y;
+                acc[nt][k].z += f0 * pv[j][nt][k].z, acc[nt][k].w += f1 * pv[j][nt][k].w;
+              }
             }
           }
         }
       }
     }
-    if (writes && orow < rows_here) {
-      const int at = tile * ROWS + orow, i = at / g, h = kvh * g + (at - i * g);
-      const int64_t out_row = (token0 + i) * a.heads + h;
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      E* out = static_cast<E*>(a.out) + out_row * D + ocol;
+    if (writes) {
+      // a fragment transposed: row lane / 4, elements (lane & 3) * 2 and the next, then 8 further
 #pragma unroll
-      for (int c = 0; c < COLS; c += 4)
-        *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<E>(acc[c] * inv, acc[c + 1] * inv),
-                                                        pack2<E>(acc[c + 2] * inv, acc[c + 3] * inv));
-      if (a.lse && ocol == 0)
-        a.lse[out_row] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+      for (int nt = 0; nt < NT; ++nt) {
+        const float i0 = sum[nt][0] > 0.f ? 1.f / sum[nt][0] : 0.f;
+        const float i1 = sum[nt][1] > 0.f ? 1.f / sum[nt][1] : 0.f;
+        const int row = nt * 8 + (lane >> 2), at = it.tile * ROWS + row;
+        const int i = at / g, h = it.kvh * g + (at - i * g);
+        E* out = static_cast<E*>(a.out) + ((it.token0 + i) * a.heads + h) * D + (lane & 3) * 2;
+#pragma unroll
+        for (int k = 0; k < F; ++k) {
+          const float4 v = acc[nt][k];
+          const uint32_t lo = transpose8x8(pack2<E>(v.x * i0, v.y * i1));
+          const uint32_t hi = transpose8x8(pack2<E>(v.z * i0, v.w * i1));
+          if (row < rows_here) {
+            *reinterpret_cast<uint32_t*>(out + (warp * F + k) * 16) = lo;
+            *reinterpret_cast<uint32_t*>(out + (warp * F + k) * 16 + 8) = hi;
+          }
+        }
+        if (a.lse && warp == 0 && lane < 4) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = nt * 8 + lane * 2 + e, x = it.tile * ROWS + r;
+            if (r < rows_here)
+              a.lse[(it.token0 + x / g) * a.heads + it.kvh * g + x % g] =
+                  top[nt][e] == -INFINITY ? -INFINITY : (top[nt][e] + log2f(sum[nt][e])) * kLn2;
+          }
+        }
+      }
     }
-    u += b_last - b_first;
-    __syncthreads();  // shared memory is free for the next item
+    __syncthreads();  // the exchange is read before the next item's
   }
+  copies_wait<0>();
 }
 
 // ---- host
@@ -438,9 +552,8 @@ size_t attend_rows_partials(const tr_attention& a) {
 
 template <typename E, int D, int NT>
 static int launch_rows(const tr_attention& a, const AttendWorkspace& ws, void* stream) {
-  constexpr int pipeline = kRowsWarps * kRowsStages * 2 * warp_keys<D>() * D * 2;
-  constexpr int joined = kRowsWarps * 8 * NT * (D + 4) * 4;
-  constexpr int smem = pipeline > joined ? pipeline : joined;
+  constexpr int smem = kRowsWarps * rows_stages<NT>() * 2 * warp_keys<D>() * D * 2 +  // stages
+                       kRowsWarps * 3 * NT * (D / 64) * 512;                          // exchange
   auto kernel = attend_rows_kernel<E, D, NT>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
