@@ -261,7 +261,20 @@ struct RowSums {  // one value or two per block of the cluster, in every block
   double v[2][8][2];
 };
 
-// The greatest of the logits in a 16-byte vector (NaN aside), and NaN made -inf in it.
+// The greatest of the logits in a 16-byte vector without NaN.
+template <typename L>
+__device__ __forceinline__ float greatest_of(const uint4& x) {
+  using P = typename std::conditional<std::is_same<L, __half>::value, __half2, __nv_bfloat162>::type;
+  const P* w = reinterpret_cast<const P*>(&x);
+  const P m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+  return fmaxf(to_f32<L>(m.x), to_f32<L>(m.y));
+}
+template <>
+__device__ __forceinline__ float greatest_of<float>(const uint4& x) {
+  return fmaxf(fmaxf(__uint_as_float(x.x), __uint_as_float(x.y)),
+               fmaxf(__uint_as_float(x.z), __uint_as_float(x.w)));
+}
+// The same, and NaN made -inf in it.
 template <typename L>
 __device__ __forceinline__ float settle(uint4& x) {
   using P = typename std::conditional<std::is_same<L, __half>::value, __half2, __nv_bfloat162>::type;
@@ -274,8 +287,7 @@ __device__ __forceinline__ float settle(uint4& x) {
     for (int j = 0; j < 8; ++j)
       if (__hisnan(e[j])) e[j] = from_f32<L>(-INFINITY);
   }
-  const P m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
-  return fmaxf(to_f32<L>(m.x), to_f32<L>(m.y));
+  return greatest_of<L>(x);
 }
 template <>
 __device__ __forceinline__ float settle<float>(uint4& x) {
@@ -283,7 +295,7 @@ __device__ __forceinline__ float settle<float>(uint4& x) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (isnan(e[j])) e[j] = -INFINITY;
-  return fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
+  return greatest_of<float>(x);
 }
 
 template <typename L>
@@ -424,6 +436,19 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
       }
     }
   };
+  // the same for the finite logits from `least` on, of which there are few: a vector's greatest first
+  const auto each_from = [&](float least, auto f) {
+    for (int v = tid; v < vectors; v += kSliceThreads) {
+      const uint4 x = slice_raw[v];
+      if (greatest_of<L>(x) < least) continue;
+      const L* e = reinterpret_cast<const L*>(&x);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float l = to_f32<L>(e[j]);
+        if (l >= least && l > -INFINITY) f(l, v * W + j);
+      }
+    }
+  };
   const float per_unit = fminf(kLog2e / div, FLT_MAX);
   const auto weight = [&](float l) { return exp2_approx((l - top) * per_unit); };
   const float top_t = top / div;
@@ -482,44 +507,61 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   const auto draw = [&](float bound_l, int bound_i, float& won_l) {
     Best best = {-INFINITY, INT32_MAX};
     float best_l = 0.f;
+    const auto ranked_above = [&](float l, int i) {
+      return l > bound_l || (l == bound_l && first + i < bound_i);
+    };
+    const auto consider = [&](float l, int i, float e) {
+      const Best b = {key_of(l, e), first + i};
+      if (b.value > best.value || (b.value == best.value && b.index < best.index))
+        best = b, best_l = l;
+    };
     if (!hot) {
-      each([&](float l, int i) {
-        if (l == top && first + i < best.index) best = {l, first + i}, best_l = l;
+      each_from(top, [&](float l, int i) {
+        if (first + i < best.index) best = {l, first + i}, best_l = l;
+      });
+    } else if (least_weight > 0.f) {
+      // those that may be heavy enough, a little below the least weight's logit
+      const float t = top_t + logf(least_weight);
+      const float least = (t - 1e-3f - fabsf(t) * 5e-7f) * div;
+      each_from(isnan(least) ? -INFINITY : least, [&](float l, int i) {
+        if (ranked_above(l, i) && heavy_enough(l)) consider(l, i, noise[i]);
       });
     } else {
-      // The logarithm in full only where its approximation comes within 1e-3 of the best so far;
-      // t by the reciprocal is within 2^-22 of |t|.
-      const float inv = fminf(1.f / div, FLT_MAX);
-      const float sure = least_weight > 0.f ? (top_t + logf(least_weight)) - 1e-3f : -INFINITY;
-      const auto consider = [&](float l, int i, float e) {
-        const float t = l * inv;
-        if (t - __logf(e) < best.value - 1e-3f - fabsf(t) * 5e-7f) return;
-        const Best b = {key_of(l, e), first + i};
-        if (b.value > best.value || (b.value == best.value && b.index < best.index))
-          best = b, best_l = l;
-      };
-      const auto ranked_above = [&](float l, int i) {
-        return l > bound_l || (l == bound_l && first + i < bound_i);
-      };
-      if (least_weight > 0.f) {
-        each([&](float l, int i) {
-          if (l * inv + fabsf(l * inv) * 5e-7f < sure || !ranked_above(l, i) || !heavy_enough(l))
-            return;
-          consider(l, i, noise[i]);
-        });
-      } else {
-        for (int i0 = tid; i0 < n; i0 += 8 * kSliceThreads) {
-          float e[8], l[8];
+      // The approximate keys of all, t log2(e) - log2(noise), the thread's greatest two kept: an
+      // exact key costs four times as much, and in a warp of 32 some lane has a new greatest at
+      // most steps.  Exact then are those within the approximation's reach of the block's
+      // greatest (errors: 2^-23 of t log2(e), 2^-21 of the logarithm).
+      float first_a = -INFINITY, second_a = -INFINITY;
+      int first_i = 0;
+      const auto approx = [&](float l, float e) { return l * per_unit - __log2f(e); };
+      for (int i0 = tid; i0 < n; i0 += 8 * kSliceThreads) {
+        float e[8], l[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int i = i0 + j * kSliceThreads;
-            l[j] = i < n ? to_f32<L>(slice[i]) : -INFINITY;
-            if (!ranked_above(l[j], i)) l[j] = -INFINITY;
-            e[j] = l[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
+        for (int j = 0; j < 8; ++j) {
+          const int i = i0 + j * kSliceThreads;
+          l[j] = i < n ? to_f32<L>(slice[i]) : -INFINITY;
+          if (!ranked_above(l[j], i)) l[j] = -INFINITY;
+          e[j] = l[j] > -INFINITY ? __ldcs(noise + i) : 1.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = approx(l[j], e[j]);
+          second_a = fmaxf(second_a, fminf(first_a, x));
+          if (x > first_a) first_a = x, first_i = i0 + j * kSliceThreads;
+        }
+      }
+      const float most_a = block_max(first_a);
+      const float within = most_a - 2e-3f - 1e-6f * fabsf(most_a);
+      if (!(first_a < within)) {
+        if (second_a < within) {
+          consider(to_f32<L>(slice[first_i]), first_i, noise[first_i]);
+        } else {
+          for (int i = tid; i < n; i += kSliceThreads) {
+            const float l = to_f32<L>(slice[i]);
+            if (!(l > -INFINITY) || !ranked_above(l, i)) continue;
+            const float e = noise[i];
+            if (!(approx(l, e) < within)) consider(l, i, e);
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (l[j] > -INFINITY) consider(l[j], i0 + j * kSliceThreads, e[j]);
         }
       }
     }
@@ -547,12 +589,12 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
 
   if (limited) {
     uint32_t* all = cluster.map_shared_rank(total, 0);
-    // Gathers the tokens that `takes(l)` in block 0, if at most kCandidates, and ranks them in its
+    // Gathers the tokens from `least` on that `takes(l)` in block 0, if at most kCandidates, and ranks them in its
     // own_l, own_i; cluster barriers.  Returns their number.
-    const auto gather = [&](auto takes) {
+    const auto gather = [&](float least, auto takes) {
       if (tid == 0) sh_count = 0;
       __syncthreads();
-      each([&](float l, int i) {
+      each_from(least, [&](float l, int i) {
         if (!takes(l)) return;
         const int at = atomicAdd(&sh_count, 1);
         if (at < kCandidates) own_l[at] = l, own_i[at] = first + i;
@@ -608,7 +650,7 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
     if ((by_count || by_mass) && reach < kBins - 1) {
       // a compare first, one step too low, and the bins' exact test for what passes
       const float edge = top - (reach + 2) / bins_per_logit;
-      const int m = gather([&](float l) { return l >= edge && bin_of(l) <= reach; });
+      const int m = gather(edge, [&](float l) { return bin_of(l) <= reach; });
       if (m <= kCandidates) {
         if (rank != 0) return;
         // ---- all limits on the ranked list
@@ -650,7 +692,7 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
         else below = mid, over_below = (int)over.y;
       }
       if (at - below > 1) {
-        const int m = gather([&](float l) {
+        const int m = gather(-INFINITY, [&](float l) {
           const uint32_t key = order_key(l);
           return key > below && key <= at;
         });
