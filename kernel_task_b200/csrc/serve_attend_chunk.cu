@@ -37,7 +37,7 @@ constexpr int kSubRows = 128, kTileRows = 2 * kSubRows;
 constexpr int kChunkThreads = 12 * 32;
 constexpr int kMinChunkUnits = 6;  // units a grid block takes at least
 constexpr int kItemUnits = 3;
-constexpr unsigned kChunkWaitPolls = 1u << 16;  // of about 20 us
+constexpr unsigned kChunkWaitPolls = 1u << 19;  // of 2638 cycles each: about 0.7 s
 
 template <int D>
 __host__ __device__ constexpr int ring_slots() {
@@ -74,6 +74,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+}
+
+// One try_wait without a time limit of its own: the warp is suspended for up to 2638 cycles
+// (measured; with a limit of 20 us given, 7814, and 3 % slower here).
+__device__ __forceinline__ bool mbar_try_once(uint32_t mbar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(mbar), "r"(parity)
+      : "memory");
+  return done != 0;
 }
 
 // tcgen05.mma with A in tensor memory, issued by one elected lane of a converged warp
@@ -309,12 +322,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t qbase = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t ring = qbase + 2 * QBYTES;
   volatile int* abort = &sh_abort;
-  // Bounded wait of a whole warp.  try_wait suspends the warp, up to some 20 us at a time, which
-  // leaves the issue slots to the softmax (polling: 4 % faster over long contexts with a head_dim
-  // of 128, 9 % slower with 64 and over short prompts).
+  // Bounded wait of a whole warp.  try_wait suspends the warp, which leaves the issue slots to the
+  // softmax (polling with test_wait: 4 % faster over long contexts with a head_dim of 128, 15 %
+  // slower with 64 and over short prompts).  The loop is as plain as can be: a first try ahead
+  // of it, or a clock in it, cost the same 15 %.
   const auto wait = [&](int b, uint32_t parity) {
     bool ok = true;
-    for (unsigned i = 0; ok && !mbar_try(bar(b), parity); ++i) {
+    for (unsigned i = 0; ok && !mbar_try_once(bar(b), parity); ++i) {
       if (*abort) ok = false;
       if (i >= wait_polls) {
         *abort = 1;
@@ -578,11 +592,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             // P of the block before has been read from this half
             if (blocks[t] && !(ok = wait(B_PRODUCT + 2 * t + half, (blocks[t] - 1) & 1))) break;
             tc_fence_after();
+            // descriptors by adding to one: no address field overflows, and the sums of constants
+            // stay in uniform registers (8192 prompt tokens: 539 us without, 523 with)
+            const uint64_t queries = desc_sw128(qbase + t * QBYTES);
+            const uint64_t block = desc_sw128(keys + half * (64 * 128));
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t in = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-              umma_one(tmem + t * 128 + half * 64, desc_sw128(qbase + t * QBYTES + in),
-                       desc_sw128(keys + half * (64 * 128) + in), idesc_s, ks > 0);
+              const int in = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+              umma_one(tmem + t * 128 + half * 64, queries + in / 16, block + in / 16, idesc_s,
+                       ks > 0);
             }
             commit_one(bar(B_SCORES + 2 * t + half));
           }

@@ -237,7 +237,7 @@ static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, in
   attr.val.clusterDim.x = blocks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;  // a single block is a cluster of its own
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
   if (e != cudaSuccess) {
     set_error("%s launch: %s", what, cudaGetErrorString(e));
