@@ -60,11 +60,34 @@ void check(int st, const char* what) {
   if (st != TR_OK) raise_status(st, what);
 }
 
+// The small outputs of a call.  As a rule they share one allocation (an allocation costs a
+// microsecond of the host, a tensor on its storage a tenth); `apart`, for the registered torch
+// ops, whose outputs may not share storage, each gets its own.
+class Outputs {
+ public:
+  Outputs(int64_t bytes, const at::Tensor& like, bool apart) : options_(like.options()) {
+    if (!apart) all_ = at::empty({bytes}, options_.dtype(at::kByte));
+  }
+  // n values of `type`, at byte `at` of the shared allocation
+  at::Tensor take(int64_t at, int64_t n, at::ScalarType type) const {
+    if (!all_.defined()) return at::empty({n}, options_.dtype(type));
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all_.storage()), all_.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+  }
+
+ private:
+  at::TensorOptions options_;
+  at::Tensor all_;
+};
+
 // ---- step plan
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_step(
     const at::Tensor& lens, const at::Tensor& brings, const at::Tensor& tables,
     const at::Tensor& free_pages, const at::Tensor& free_count, int64_t page_size, int64_t tokens,
-    bool inplace) {
+    bool inplace, bool apart) {
   const char* op = "plan_step";
   need(op, "lens", lens, at::kInt, 1, lens);
   const int64_t R = lens.size(0);
@@ -79,12 +102,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   if (tables.size(1) > INT32_MAX) refuse(op, "too many table columns");
   const c10::cuda::CUDAGuard guard(lens.device());
   const at::AutoDispatchBelowADInplaceOrView no_grad;
-  const auto ints = lens.options();
-  at::Tensor slots = at::empty({tokens}, ints.dtype(at::kLong));
-  at::Tensor positions = at::empty({tokens}, ints), starts = at::empty({R + 1}, ints),
-             granted = at::empty({R}, ints);
-  at::Tensor lens_out = inplace ? lens : at::empty({R}, ints);
-  at::Tensor count_out = inplace ? free_count : at::empty({1}, ints);
+  // slots, positions (from a multiple of 16 bytes on), starts, granted, lens, count
+  const int64_t at_positions = (tokens * 8 + 15) / 16 * 16, at_starts = at_positions + tokens * 4;
+  const Outputs outputs(at_starts + (3 * R + 2) * 4, lens, apart);
+  const at::Tensor slots = outputs.take(0, tokens, at::kLong);
+  const at::Tensor positions = outputs.take(at_positions, tokens, at::kInt);
+  const at::Tensor starts = outputs.take(at_starts, R + 1, at::kInt);
+  const at::Tensor granted = outputs.take(at_starts + (R + 1) * 4, R, at::kInt);
+  const at::Tensor lens_out =
+      inplace ? lens : outputs.take(at_starts + (2 * R + 1) * 4, R, at::kInt);
+  const at::Tensor count_out =
+      inplace ? free_count : outputs.take(at_starts + (3 * R + 1) * 4, 1, at::kInt);
   check(tr_plan_step(lens.data_ptr<int32_t>(), brings.data_ptr<int32_t>(), R,
                      tables.data_ptr<int32_t>(), row_stride(tables), (int32_t)tables.size(1),
                      free_pages.data_ptr<int32_t>(), free_pages.size(0),
@@ -361,7 +389,7 @@ std::pair<OptTensor, OptTensor> residual_norm(const OptTensor& y, const at::Tens
 std::pair<at::Tensor, at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor& noise,
                                                 const at::Tensor& temperature,
                                                 const OptTensor& top_k, const OptTensor& top_p,
-                                                const OptTensor& min_p) {
+                                                const OptTensor& min_p, bool apart) {
   const char* op = "sample_tokens";
   if (dtype_code(logits.scalar_type()) < 0)
     refuse(op, "logits must be float32, float16 or bfloat16");
@@ -378,8 +406,9 @@ std::pair<at::Tensor, at::Tensor> sample_tokens(const at::Tensor& logits, const 
   const c10::cuda::CUDAGuard guard(logits.device());
   const at::Tensor lc = V > 1 && logits.stride(1) != 1 ? logits.contiguous() : logits;
   const at::Tensor nc = V > 1 && noise.stride(1) != 1 ? noise.contiguous() : noise;
-  at::Tensor tokens = at::empty({R}, logits.options().dtype(at::kLong));
-  at::Tensor logprobs = at::empty({R}, logits.options().dtype(at::kFloat));
+  const Outputs outputs(R * 12, logits, apart);
+  const at::Tensor tokens = outputs.take(0, R, at::kLong);
+  const at::Tensor logprobs = outputs.take(R * 8, R, at::kFloat);
   check(tr_sample(lc.data_ptr(), dtype_code(lc.scalar_type()), row_stride(lc),
                   nc.data_ptr<float>(), row_stride(nc), temperature.data_ptr<float>(),
                   top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr,
@@ -395,7 +424,7 @@ std::pair<at::Tensor, at::Tensor> sample_tokens(const at::Tensor& logits, const 
 void bind_serving(py::module_& m) {
   m.def("plan_step", &plan_step, py::arg("lens"), py::arg("new"), py::arg("tables"),
         py::arg("free"), py::arg("free_count"), py::arg("page_size"), py::arg("tokens"),
-        py::arg("inplace") = false);
+        py::arg("inplace") = false, py::arg("apart") = false);
   m.def("release_pages", &release_pages, py::arg("lens"), py::arg("finished"), py::arg("tables"),
         py::arg("free"), py::arg("free_count"), py::arg("page_size"));
   m.def("append_kv", &append_kv, py::arg("k"), py::arg("v"), py::arg("k_pages"),
@@ -408,7 +437,7 @@ void bind_serving(py::module_& m) {
         py::arg("kind"), py::arg("eps"), py::arg("residual_scale"), py::arg("branch_scale"));
   m.def("sample_tokens", &sample_tokens, py::arg("logits"), py::arg("noise"),
         py::arg("temperature"), py::arg("top_k") = py::none(), py::arg("top_p") = py::none(),
-        py::arg("min_p") = py::none());
+        py::arg("min_p") = py::none(), py::arg("apart") = false);
 }
 
 }  // namespace trr_torch

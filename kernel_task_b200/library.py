@@ -31,6 +31,7 @@ from typing import Optional
 import torch
 
 from . import serve as _serve
+from ._native import binding
 from .ring import consume_add as _consume_add
 from .ring import consume_silu_mul as _consume_silu_mul
 from .spec import TRSpec
@@ -136,7 +137,7 @@ def plan_step(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free:
               free_count: torch.Tensor, page_size: int, tokens: int) -> tuple[
                   torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                   torch.Tensor]:
-    return tuple(_serve.plan_step(lens, new, tables, free, free_count, page_size, tokens))
+    return binding().plan_step(lens, new, tables, free, free_count, page_size, tokens, apart=True)
 
 
 @plan_step.register_fake
@@ -190,7 +191,7 @@ def _(y, h, post, pre, gate, post_bias, pre_bias, kind, eps, residual_scale, bra
 def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor,
                   top_k: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
                   min_p: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
-    return _serve.sample_tokens(logits, noise, temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    return binding().sample_tokens(logits, noise, temperature, top_k, top_p, min_p, apart=True)
 
 
 @sample_tokens.register_fake

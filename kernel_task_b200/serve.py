@@ -27,7 +27,8 @@ from ._native import binding
 
 
 class StepPlan(NamedTuple):
-    """What one step's tokens need; the tokens are numbered request by request."""
+    """What one step's tokens need; the tokens are numbered request by request.  The tensors of
+    a plan share one allocation."""
 
     slots: torch.Tensor       # int64 [tokens], -1 where there is no token or its request is refused
     positions: torch.Tensor   # int32 [tokens], the token's position in its request, or -1
