@@ -87,6 +87,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     float16 and bfloat16 with head_dim 64 or 128 run on tensor cores, other multiples of 8 up to
     256 and float32 on a general kernel.  The page size is a power of two up to 1024.
+    Values of a request's own tokens have to be finite: a later token's infinity or NaN may reach
+    earlier tokens of the same call; what lies past the length may be anything.
     """
     out, lse = binding().paged_attention(q, k_pages, v_pages, tables, lens, starts, scale,
                                          return_lse)
