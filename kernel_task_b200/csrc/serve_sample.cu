@@ -328,6 +328,8 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
 
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+  // announce that this block runs; the wait stands before the first store into another's memory
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / ranks;
   const int V = a.vocab;
@@ -420,7 +422,9 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
       slice_raw[v] = x;
     }
   }
-  float top = (float)over_cluster(block_max(greatest), 0., most).x;
+  const float block_top = block_max(greatest);
+  asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");  // every block has started
+  float top = (float)over_cluster(block_top, 0., most).x;
   if (top == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
