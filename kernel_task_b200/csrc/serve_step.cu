@@ -216,15 +216,20 @@ __global__ void __launch_bounds__(kStepThreads, 1) release_pages_kernel(const Re
   }
 }
 
-// One launch of a single cluster of `blocks`.
+// One launch of a single cluster of `blocks`, with ints_per_request of shared memory a request and
+// one more.  The default limit of 48 KB is for the kernel's own variables and these together; past
+// 40 KB it is raised, to the same size whatever the call, so that calls of several threads do not
+// lower it under one another.
 template <typename Args>
 static int launch_cluster(void (*kernel)(Args), const Args& args, int blocks, int threads,
-                          size_t smem, void* stream, const char* what) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                          int ints_per_request, void* stream, const char* what) {
+  const size_t smem = (ints_per_request * (size_t)args.requests + 1) * sizeof(int32_t);
+  if (smem > 40 * 1024) {
+    const int most = (ints_per_request * TR_STEP_MAX_REQUESTS + 1) * (int)sizeof(int32_t);
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) {
-      set_error("%s: %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(e));
+      set_error("%s: %d bytes of shared memory: %s", what, most, cudaGetErrorString(e));
       return TR_ERR_CUDA;
     }
   }
@@ -395,8 +400,7 @@ extern "C" int tr_plan_step(const int32_t* lens, const int32_t* new_tokens, int6
   const int64_t work = std::max(requests, tokens / 4);
   const int blocks = tokens > 8 * kStepThreads ? 8 : 1;
   const int threads = blocks > 1 || work > 512 ? kStepThreads : work > 256 ? 512 : 256;
-  return launch_cluster(plan_step_kernel, a, blocks, threads, (3 * requests + 1) * sizeof(int32_t),
-                        stream, "tr_plan_step");
+  return launch_cluster(plan_step_kernel, a, blocks, threads, 3, stream, "tr_plan_step");
 }
 
 extern "C" int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t requests,
@@ -409,8 +413,8 @@ extern "C" int tr_release_pages(int32_t* lens, const int32_t* finished, int64_t 
   ReleaseArgs a = {lens, finished, tables, table_stride, free_pages, free_count, pool,
                    (int)requests, columns, page_size};
   const int blocks = requests * columns > 4 * kStepThreads ? 8 : 1;
-  return launch_cluster(release_pages_kernel, a, blocks, kStepThreads, requests * sizeof(int32_t),
-                        stream, "tr_release_pages");
+  return launch_cluster(release_pages_kernel, a, blocks, kStepThreads, 1, stream,
+                        "tr_release_pages");
 }
 
 extern "C" int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride,

@@ -4,14 +4,58 @@ the sizes at which launches change shape, extreme parameters, and state that out
 Tolerances are those of test_serve.py."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
+import numpy as np
 import pytest
 import torch
 
 import kernel_task_b200 as trb
-from test_serve import check_sample, i32, sample_inputs
+from test_serve import check_plan, check_sample, i32, make_pool, sample_inputs
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
+TESTS = Path(__file__).resolve().parent
+
+
+def in_fresh_process(call, **env):
+    """Runs `call` of this file where no earlier call has raised a limit or kept a workspace."""
+    code = f"import sys; sys.path[:0] = [{str(TESTS)!r}, {str(TESTS.parent)!r}]\n" \
+           f"import test_serve_edges as t\nt.{call}"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, **env})
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------------------ step plan
+def plans_of(sizes):
+    for requests in sizes:
+        check_plan([1] * requests, [1] * requests, 16, 2, requests)
+        check_plan([16] * requests, [1] * requests, 16, 2, requests)
+
+
+def releases_of(sizes):
+    for requests in sizes:
+        lens = [17] * requests
+        tables, free, total = make_pool(lens, 16, 2, 3)
+        pool = np.full(total, -1, np.int32)
+        pool[:3] = free
+        d = dict(lens=i32(lens), tables=i32(tables), free=i32(pool), count=i32([3]))
+        trb.release_pages(d["lens"], i32([1] * requests), d["tables"], d["free"], d["count"], 16)
+        assert d["free"].cpu().tolist() == list(free) + tables.flatten().tolist()
+        assert int(d["count"]) == total and not d["lens"].any()
+
+
+@gpu
+@pytest.mark.parametrize("call", ["plans_of([4074, 4073, 4095, 4096, 16384, 4095])",
+                                  "plans_of([4095])",
+                                  "releases_of([12225, 12224, 12288, 12289, 16384, 12288])",
+                                  "releases_of([12288])"])
+def test_requests_where_shared_memory_passes_the_default(call):
+    in_fresh_process(call)
 
 
 # ------------------------------------------------------------------------------- sampling
