@@ -327,10 +327,12 @@ int tr_residual_norm(const tr_norm* n, void* stream);
  *   of these the ones of at least min_p times the greatest probability;
  * the greatest always stays unless it is -inf.  The token is the kept one with the greatest
  * t - log(noise), noise [rows][vocab] ~ Exp(1), which draws it with its probability among the
- * kept; where temperature <= 0 the one with the greatest t; ties go to the lower index.  NaN
- * logits count as -inf; where logits are +inf these share all the probability.  tokens[row] is -1 when every logit is -inf.  logprobs[row] (may be
- * NULL) is the log of the token's probability in the softmax of t over the whole row, -inf with
- * token -1.  top_k, top_p and min_p may be NULL (no such limit).                             */
+ * kept; where temperature <= 0 the one with the greatest t.  Ranks and cuts are those of the
+ * logits, also where t no longer tells them apart (an infinite temperature draws evenly among
+ * what the limits keep); ties of logits go to the lower index.  NaN logits count as -inf; where
+ * logits are +inf these share all the probability.  tokens[row] is -1 when every logit is -inf.
+ * logprobs[row] (may be NULL) is the log of the token's probability in the softmax of t over the
+ * whole row, -inf with token -1.  top_k, top_p and min_p may be NULL (no such limit).        */
 int tr_sample(const void* logits, int32_t dtype, int64_t logits_stride, const float* noise,
               int64_t noise_stride, const float* temperature, const int32_t* top_k,
               const float* top_p, const float* min_p, int64_t rows, int64_t vocab,

@@ -38,9 +38,6 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // Masses are summed as whole numbers of 2^-40 of the greatest token's, so that the sums do not
 // depend on the order of the atomics.
 constexpr float kMassUnit = 1099511627776.f;  // 2^40
-__device__ __forceinline__ float weight_of(float t, float top) {
-  return t == top ? 1.f : expf(t - top);
-}
 __device__ __forceinline__ unsigned long long mass_of(float w) {
   return (unsigned long long)llrintf(w * kMassUnit);
 }
@@ -89,9 +86,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const float div = hot ? heat : 1.f;
   bool infinite = false;  // infinite logits share all the probability
   const auto value = [&](int i) {
-    const float t = to_f32<L>(logits[i]) / div;
-    if (infinite) return t == INFINITY ? 0.f : -INFINITY;
-    return isnan(t) ? -INFINITY : t;
+    const float l = to_f32<L>(logits[i]);
+    if (infinite) return l == INFINITY ? 0.f : -INFINITY;
+    return isnan(l) ? -INFINITY : l;
   };
   Best best = {-INFINITY, INT32_MAX};
   for (int i = tid; i < V; i += kSampleThreads) best = better(best, {value(i), i});
@@ -108,8 +105,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     }
     return;
   }
+  // t less the greatest t; -inf stays so under an infinite temperature
+  const auto below_top = [&](float l) {
+    return l == top ? 0.f : l == -INFINITY ? -INFINITY : l / div - top / div;
+  };
+  const auto weight = [&](float l) { return expf(below_top(l)); };
   double z = 0.;
-  for (int i = tid; i < V; i += kSampleThreads) z += weight_of(value(i), top);
+  for (int i = tid; i < V; i += kSampleThreads) z += weight(value(i));
   z = warp_sum(z);
   if ((tid & 31) == 0) dpart[tid >> 5] = z;
   __syncthreads();
@@ -148,12 +150,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       const uint32_t least = cut;
       const unsigned long long least_ties = ties;
       // mass of what top-k keeps
-      if (tid == 0) hist[0] = k < V ? least_ties * mass_of(weight_of(key_value(least), top)) : 0;
+      if (tid == 0) hist[0] = k < V ? least_ties * mass_of(weight(key_value(least))) : 0;
       __syncthreads();
       unsigned long long mine = 0;
       for (int i = tid; i < V; i += kSampleThreads) {
-        const float t = value(i);
-        if (k == V || order_key(t) > least) mine += mass_of(weight_of(t, top));
+        const float l = value(i);
+        if (k == V || order_key(l) > least) mine += mass_of(weight(l));
       }
       mine = warp_sum(mine);
       if ((tid & 31) == 0) atomicAdd(&hist[0], mine);
@@ -166,15 +168,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         for (int b = tid; b < 256; b += kSampleThreads) hist[b] = 0;
         __syncthreads();
         for (int i = tid; i < V; i += kSampleThreads) {
-          const float t = value(i);
-          const uint32_t key = order_key(t);
+          const float l = value(i);
+          const uint32_t key = order_key(l);
           if ((k == V || key > least) &&
               (shift == 24 || (key >> (shift + 8)) == (chosen >> (shift + 8))))
-            atomicAdd(&hist[(key >> shift) & 255], mass_of(weight_of(t, top)));
+            atomicAdd(&hist[(key >> shift) & 255], mass_of(weight(l)));
         }
         if (tid == 0 && k < V && (shift == 24 || (least >> (shift + 8)) == (chosen >> (shift + 8))))
           atomicAdd(&hist[(least >> shift) & 255],
-                    least_ties * mass_of(weight_of(key_value(least), top)));
+                    least_ties * mass_of(weight(key_value(least))));
         __syncthreads();
         if (tid == 0) {
           int b = 255, last = -1;
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         above = sh_left;
         __syncthreads();
       }
-      const double w = (double)mass_of(weight_of(key_value(chosen), top));
+      const double w = (double)mass_of(weight(key_value(chosen)));
       const double want = w > 0. ? ceil((target - (double)above) / w) : 1.;
       const unsigned long long most = chosen == least && k < V ? least_ties : (unsigned long long)V;
       cut = chosen;
@@ -219,12 +221,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     const float least_weight = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
     best = {-INFINITY, INT32_MAX};
     for (int i = tid; i < V; i += kSampleThreads) {
-      const float t = value(i);
-      if (t == -INFINITY) continue;
-      const uint32_t key = order_key(t);
+      const float l = value(i);
+      if (l == -INFINITY) continue;
+      const uint32_t key = order_key(l);
       if (key < cut || (key == cut && i > cut_index)) continue;
-      if (!(weight_of(t, top) >= least_weight) && t != top) continue;
-      float s = t - logf(noise[i]);
+      if (!(weight(l) >= least_weight) && l != top) continue;
+      float s = l / div - logf(noise[i]);
       if (isnan(s)) s = -INFINITY;
       best = better(best, {s, i});
     }
@@ -232,8 +234,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   }
   if (tid == 0) {
     a.tokens[row] = best.index;
-    const float t = value(best.index);
-    if (a.logprobs) a.logprobs[row] = (t == top ? 0.f : t - top) - logf((float)z);
+    if (a.logprobs) a.logprobs[row] = below_top(value(best.index)) - logf((float)z);
   }
 }
 
@@ -464,7 +465,8 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
       }
     }
   };
-  const float per_unit = fminf(kLog2e / div, FLT_MAX);
+  // above 0 under an infinite temperature too, so that the weight of -inf stays 0 and no NaN
+  const float per_unit = fmaxf(fminf(kLog2e / div, FLT_MAX), FLT_TRUE_MIN);
   const auto weight = [&](float l) { return exp2_approx((l - top) * per_unit); };
   const float top_t = top / div;
 

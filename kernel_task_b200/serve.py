@@ -126,8 +126,9 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.
     kept the top_k greatest (0: all), of these the shortest run in falling order whose mass
     reaches top_p of theirs (1: all), of these the ones of at least min_p times the greatest.
     The token is the kept one with the greatest t - log(noise), which draws it with its
-    probability among the kept, or at temperature 0 the one with the greatest logit.  Ties go to
-    the lower index everywhere.  The greatest token is always kept; NaN logits count as -inf; a
+    probability among the kept, or at temperature 0 the one with the greatest logit.  Ranks and
+    cuts are those of the logits, also where t no longer tells them apart: an infinite temperature
+    draws evenly among what the limits keep.  Ties of logits go to the lower index everywhere.  The greatest token is always kept; NaN logits count as -inf; a
     row of nothing but -inf gives token -1.
 
     Returns (tokens int64 [rows], logprobs float32 [rows]): the log of the token's probability

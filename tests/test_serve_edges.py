@@ -4,6 +4,7 @@ the sizes at which launches change shape, extreme parameters, and state that out
 Tolerances are those of test_serve.py."""
 from __future__ import annotations
 
+import math
 import os
 import subprocess
 import sys
@@ -14,7 +15,7 @@ import pytest
 import torch
 
 import kernel_task_b200 as trb
-from test_serve import check_plan, check_sample, i32, make_pool, sample_inputs
+from test_serve import check_plan, check_sample, f64, i32, make_pool, sample_inputs
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
@@ -77,3 +78,29 @@ def test_sample_rows_split_over_a_cluster_on_a_busy_gpu(vocab):
         got.append(trb.sample_tokens(logits, noise, heat, top_k=k, top_p=p)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@gpu
+@pytest.mark.parametrize("vocab,dtype", [(5000, torch.float32), (4999, torch.bfloat16),
+                                         (60001, torch.float32), (900001, torch.bfloat16)])
+def test_sample_infinite_temperature(vocab, dtype):
+    """Every finite logit has the same probability, -inf has none, +inf has all."""
+    logits, noise = sample_inputs(3, vocab, dtype, vocab)
+    logits[1, ::3] = -math.inf
+    logits[2, 5:40:7] = math.inf
+    heat = torch.full((3,), math.inf, device=DEV)
+    ids, logprobs = trb.sample_tokens(logits, noise, heat)
+    drawn = [logits[0] == logits[0], logits[1] > -math.inf, logits[2] == math.inf]
+    for r, shares in enumerate(drawn):
+        assert int(ids[r]) == int(torch.where(shares, noise[r].double(), math.inf).argmin())
+        n = int(shares.sum())
+        assert abs(float(logprobs[r]) + math.log(n)) <= 2e-5 * max(1.0, math.log(n))
+    for k in (1, 20, 700):
+        ids = trb.sample_tokens(logits, noise, heat, top_k=i32([k] * 3))[0]
+        half = trb.sample_tokens(logits, noise, heat, top_k=i32([2 * k] * 3),
+                                 top_p=torch.full((3,), 0.5, device=DEV))[0]
+        for r in (0, 1):
+            kept = np.argsort(-f64(logits[r]), kind="stable")[:k]
+            assert int(ids[r]) == int(half[r]) == int(kept[np.argmin(f64(noise[r])[kept])])
+    least = trb.sample_tokens(logits, noise, heat, min_p=torch.full((3,), 0.9, device=DEV))[0]
+    assert torch.equal(least, trb.sample_tokens(logits, noise, heat)[0])
