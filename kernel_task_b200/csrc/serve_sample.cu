@@ -105,10 +105,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     }
     return;
   }
-  // t less the greatest t; -inf stays so under an infinite temperature
-  const auto below_top = [&](float l) {
-    return l == top ? 0.f : l == -INFINITY ? -INFINITY : l / div - top / div;
-  };
+  // t less the greatest t, which stays finite at the top where t itself would pass fp32; -inf
+  // stays so under an infinite temperature
+  const auto below_top = [&](float l) { return l == -INFINITY ? l : (l - top) / div; };
   const auto weight = [&](float l) { return expf(below_top(l)); };
   double z = 0.;
   for (int i = tid; i < V; i += kSampleThreads) z += weight(value(i));
@@ -226,7 +225,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       const uint32_t key = order_key(l);
       if (key < cut || (key == cut && i > cut_index)) continue;
       if (!(weight(l) >= least_weight) && l != top) continue;
-      float s = l / div - logf(noise[i]);
+      float s = below_top(l) - logf(noise[i]);
       if (isnan(s)) s = -INFINITY;
       best = better(best, {s, i});
     }
@@ -468,7 +467,9 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   // above 0 under an infinite temperature too, so that the weight of -inf stays 0 and no NaN
   const float per_unit = fmaxf(fminf(kLog2e / div, FLT_MAX), FLT_TRUE_MIN);
   const auto weight = [&](float l) { return exp2_approx((l - top) * per_unit); };
-  const float top_t = top / div;
+  // t less the greatest t (of a finite logit): the logits are subtracted first, so that it is exact
+  // near the top and finite there, where t itself passes fp32 at the smallest temperatures
+  const auto below_top = [&](float l) { return (l - top) / div; };
 
   // ---- sum of the weights, and the threads' greatest in steps below the greatest
   const bool limited = hot && (k < V || p < 1.f);
@@ -508,14 +509,12 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
   const float log_z = logf((float)Z);
   const auto answer = [&](int index, float l) {
     a.tokens[row] = index;
-    if (a.logprobs) a.logprobs[row] = (l == top ? 0.f : l / div - top_t) - log_z;
+    if (a.logprobs) a.logprobs[row] = below_top(l) - log_z;
   };
-  const auto heavy_enough = [&](float l) {
-    const float t = l / div;
-    return t == top_t || expf(t - top_t) >= least_weight;
-  };
-  const auto key_of = [&](float l, float e) {  // t - log(noise), a NaN last
-    const float s = l / div - logf(e);
+  const auto heavy_enough = [&](float l) { return l == top || expf(below_top(l)) >= least_weight; };
+  // t - log(noise) less the greatest t, a NaN last
+  const auto key_of = [&](float l, float e) {
+    const float s = below_top(l) - logf(e);
     return isnan(s) ? -INFINITY : s;
   };
 
@@ -537,10 +536,12 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
         if (first + i < best.index) best = {l, first + i}, best_l = l;
       });
     } else if (least_weight > 0.f) {
-      // those that may be heavy enough, a little below the least weight's logit
-      const float t = top_t + logf(least_weight);
-      const float least = (t - 1e-3f - fabsf(t) * 5e-7f) * div;
-      each_from(isnan(least) ? -INFINITY : least, [&](float l, int i) {
+      // those that may be heavy enough, a little below the least weight's logit (roundings: 2^-22
+      // of t's distance from the top, 2^-24 each of the two logits)
+      const float t = logf(least_weight);
+      float least = top + (t - 1e-3f - fabsf(t) * 5e-7f) * div;
+      least -= (fabsf(least) + fabsf(top)) * 2e-7f;
+      each_from(least, [&](float l, int i) {
         if (ranked_above(l, i) && heavy_enough(l)) consider(l, i, noise[i]);
       });
     } else {

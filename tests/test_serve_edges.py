@@ -104,3 +104,34 @@ def test_sample_infinite_temperature(vocab, dtype):
             assert int(ids[r]) == int(half[r]) == int(kept[np.argmin(f64(noise[r])[kept])])
     least = trb.sample_tokens(logits, noise, heat, min_p=torch.full((3,), 0.9, device=DEV))[0]
     assert torch.equal(least, trb.sample_tokens(logits, noise, heat)[0])
+
+
+@gpu
+@pytest.mark.parametrize("vocab,dtype", [(5000, torch.float32), (4999, torch.bfloat16),
+                                         (900001, torch.bfloat16)])
+@pytest.mark.parametrize("temperature", [1e-36, 1e-38, 1e-45])
+def test_sample_temperatures_at_which_t_passes_fp32(vocab, dtype, temperature):
+    """The greatest logit has all the probability (shared among its equals)."""
+    logits, noise = sample_inputs(3, vocab, dtype, vocab)
+    logits[2] -= 100
+    heat = torch.full((3,), temperature, device=DEV)
+    least = torch.full((3,), 0.1, device=DEV)
+    for limits in (dict(), dict(top_k=i32([5] * 3)), dict(min_p=least), dict(top_p=least)):
+        ids, logprobs = trb.sample_tokens(logits, noise, heat, **limits)
+        for r in range(3):
+            top = logits[r] == logits[r].max()
+            assert int(ids[r]) == int(torch.where(top, noise[r].double(), math.inf).argmin()) \
+                or "top_p" in limits and bool(top[ids[r]])
+            assert abs(float(logprobs[r]) + math.log(int(top.sum()))) <= 2e-5
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [-3e4, 3e4])
+def test_sample_min_p_of_logits_far_from_zero(shift, dtype):
+    """The search's lower bound is rounded at the size of the logits, not of their differences."""
+    logits, noise = sample_inputs(4, 20000, dtype, 11, scale=300.0)
+    logits += shift
+    heat = torch.tensor([0.01, 1.0, 40.0, 300.0], device=DEV)
+    least = torch.tensor([0.5, 0.01, 0.3, 0.05], device=DEV)
+    check_sample(logits, noise, heat, min_p=least)
