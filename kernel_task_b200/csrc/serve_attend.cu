@@ -45,7 +45,9 @@ __global__ void __launch_bounds__(128) attend_generic_kernel(const tr_attention 
       if (held && d < a.head_dim) s = fmaf(qf[i], to_f32<E>(k[d]), s);
     }
     s = warp_sum(s);
-    const float top = fmaxf(m, s), keep = __expf(m - top), p = __expf(s - top);
+    // scores may be -inf (a product that passes fp32): no difference of infinities
+    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
+    const float keep = __expf(m - base), p = __expf(s - base);
     m = top;
     l = l * keep + p;
 #pragma unroll
@@ -54,14 +56,14 @@ __global__ void __launch_bounds__(128) attend_generic_kernel(const tr_attention 
       o[i] = o[i] * keep + (held && d < a.head_dim ? p * to_f32<E>(v[d]) : 0.f);
     }
   }
-  const float inv = keys > 0 ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key, or scores of nothing but -inf
   E* out = static_cast<E*>(a.out) + (t * a.heads + h) * a.head_dim;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int d = i * 32 + lane;
     if (d < a.head_dim) out[d] = from_f32<E>(o[i] * inv);
   }
-  if (a.lse && lane == 0) a.lse[t * a.heads + h] = keys > 0 ? m + logf(l) : -INFINITY;
+  if (a.lse && lane == 0) a.lse[t * a.heads + h] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 template <typename E>

@@ -15,7 +15,8 @@ import pytest
 import torch
 
 import kernel_task_b200 as trb
-from test_serve import check_plan, check_sample, f64, i32, make_pool, sample_inputs
+from test_serve import (attention_case, check_attention, check_plan, check_sample, f64, i32, make_pool,
+                        sample_inputs)
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
@@ -57,6 +58,19 @@ def releases_of(sizes):
                                   "releases_of([12288])"])
 def test_requests_where_shared_memory_passes_the_default(call):
     in_fresh_process(call)
+
+
+# ------------------------------------------------------------------------------ attention
+@gpu
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 40), (torch.bfloat16, 40),
+                                       (torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_attention_scores_that_pass_fp32_downwards(new, dtype, dim):
+    """The first keys' scores are -inf in fp32: their probability is 0, as in 64 bits."""
+    q, kp, vp, tables, lens, starts = attention_case([100], [new], 4, 2, dim, 16, dtype)
+    kp[int(tables[0, 0]), :, :3, 0] = -3e38
+    kp[int(tables[0, 5]), :, 2, 0] = -3e38
+    check_attention((q.abs() + 1, kp, vp, tables, lens, starts))
 
 
 # ------------------------------------------------------------------------------- sampling
