@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
       if (writes && live && a.lse)
-        a.lse[out_row] = m > -INFINITY ? (m + log2f(l)) * kLn2 : -INFINITY;
+        a.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       tc_fence_before();  // O is free for the next item once its B_PROBS arrive
     }
   } else if (warp == 8) {

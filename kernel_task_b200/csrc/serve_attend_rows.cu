@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attend_rows_kernel(const tr_a
             const int r = nt * 8 + lane * 2 + e, x = it.tile * ROWS + r;
             if (r < rows_here)
               a.lse[(it.token0 + x / g) * a.heads + it.kvh * g + x % g] =
-                  top[nt][e] == -INFINITY ? -INFINITY : (top[nt][e] + log2f(sum[nt][e])) * kLn2;
+                  sum[nt][e] == 0.f ? -INFINITY : (top[nt][e] + log2f(sum[nt][e])) * kLn2;
           }
         }
       }

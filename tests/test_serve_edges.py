@@ -73,6 +73,21 @@ def test_attention_scores_that_pass_fp32_downwards(new, dtype, dim):
     check_attention((q.abs() + 1, kp, vp, tables, lens, starts))
 
 
+@gpu
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_attention_log_sum_of_a_nan_row_is_nan(new, dim):
+    """-inf would say that the row saw nothing, and a join by log-sums would drop the NaN."""
+    args = attention_case([100], [new], 4, 2, dim, 16, torch.bfloat16)
+    want, want_lse = trb.paged_attention(*args, return_lse=True)
+    q = args[0].clone()
+    q[0, 1] = math.nan
+    out, lse = trb.paged_attention(q, *args[1:], return_lse=True)
+    assert out[0, 1].isnan().all() and lse[0, 1].isnan()
+    out[0, 1], lse[0, 1] = want[0, 1], want_lse[0, 1]
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 # ------------------------------------------------------------------------------- sampling
 @gpu
 @pytest.mark.parametrize("vocab", [2049, 4097, 8193, 16391])
