@@ -110,6 +110,9 @@ __device__ __forceinline__ void norm_row(float (&f)[N][V], const E* weight, cons
   if constexpr (LAYER) {
     d = sums.y * inv_width;
     s = fmaf(-d, d, s);
+    // of a row of one value what is left is rounding, of either sign: below 0 it may pass a small
+    // eps (a NaN stays)
+    s = s < 0.f ? 0.f : s;
   }
   const float r = rsqrtf(s + eps);
 #pragma unroll

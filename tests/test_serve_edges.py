@@ -15,8 +15,8 @@ import pytest
 import torch
 
 import kernel_task_b200 as trb
-from test_serve import (attention_case, check_attention, check_plan, check_sample, f64, i32, make_pool,
-                        sample_inputs)
+from test_serve import (attention_case, check_attention, check_plan, check_sample, f64, gen, i32,
+                        make_pool, sample_inputs)
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
@@ -86,6 +86,23 @@ def test_attention_log_sum_of_a_nan_row_is_nan(new, dim):
     assert out[0, 1].isnan().all() and lse[0, 1].isnan()
     out[0, 1], lse[0, 1] = want[0, 1], want_lse[0, 1]
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+# ---------------------------------------------------------------------------------- norms
+@gpu
+@pytest.mark.parametrize("width", [33, 768, 1000, 1920, 4096, 5001, 14336, 32760])
+@pytest.mark.parametrize("eps", [1e-5, 1e-12])
+def test_layer_norm_of_rows_of_one_value(width, eps):
+    """Nothing is left but the bias.  The mean is off by c 2^-22 at most (a tree of sums) and the
+    mean of the differences by 2^-20 of that, times 1 / sqrt(eps)."""
+    for size in (1.0, 1e4, 1e6):
+        c = torch.rand(300, generator=gen(width), device=DEV) * size
+        h = c[:, None].expand(300, width).contiguous()
+        h[0, 0] = math.nan
+        w, b = torch.ones(width, device=DEV), torch.full((width,), 0.25, device=DEV)
+        x = trb.residual_norm(None, h, pre=w, pre_bias=b, kind="layer", eps=eps)[1]
+        assert x[0].isnan().all()
+        assert float((x[1:] - 0.25).abs().max()) <= 1e-6 + size * 2.0 ** -42 / eps ** 0.5
 
 
 # ------------------------------------------------------------------------------- sampling
