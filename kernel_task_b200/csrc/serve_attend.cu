@@ -119,7 +119,7 @@ static int check_attention(const tr_attention* a) {
     return TR_ERR_UNSUPPORTED;
   }
   if ((int64_t)a->columns * a->page_size > (int64_t)1 << 30 ||
-      a->tokens * a->heads > (int64_t)1 << 31 || a->requests > (int64_t)1 << 20 ||
+      a->tokens > INT32_MAX || a->tokens * a->heads > (int64_t)1 << 31 || a->requests > (int64_t)1 << 20 ||
       a->pages > INT32_MAX ||
       (double)a->pages * a->kv_heads * a->page_size >= 4294967295.) {
     set_error("tr_paged_attention: too large (a request's cache up to 2^30 tokens, tokens x heads "
@@ -132,6 +132,10 @@ static int check_attention(const tr_attention* a) {
       (a->pages > 0 && (!a->k_pages || !a->v_pages))) {
     set_error("tr_paged_attention: null pointer");
     return TR_ERR_INVALID;
+  }
+  if (((uintptr_t)a->tables | (uintptr_t)a->lens | (uintptr_t)a->starts | (uintptr_t)a->lse) & 3) {
+    set_error("tr_paged_attention: a pointer is not aligned to its elements");
+    return TR_ERR_ALIGN;
   }
   const int eb = element_bytes(a->dtype);
   if ((((uintptr_t)a->q | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->out) & 15) ||

@@ -370,6 +370,11 @@ static int check_step(const char* what, int64_t requests, const void* a, const v
     set_error("%s: null pointer", what);
     return TR_ERR_INVALID;
   }
+  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)tables | (uintptr_t)free_pages |
+       (uintptr_t)free_count) & 3) {
+    set_error("%s: a pointer is not aligned to its elements", what);
+    return TR_ERR_ALIGN;
+  }
   return TR_OK;
 }
 
@@ -390,6 +395,11 @@ extern "C" int tr_plan_step(const int32_t* lens, const int32_t* new_tokens, int6
       (tokens > 0 && (!slots || !positions))) {
     set_error("tr_plan_step: null output");
     return TR_ERR_INVALID;
+  }
+  if ((((uintptr_t)positions | (uintptr_t)starts | (uintptr_t)lens_out | (uintptr_t)granted |
+        (uintptr_t)free_count_out) & 3) || ((uintptr_t)slots & 7)) {
+    set_error("tr_plan_step: an output is not aligned to its elements");
+    return TR_ERR_ALIGN;
   }
   StepArgs a = {lens, new_tokens, tables, table_stride, free_pages, free_count, slots, positions,
                 starts, lens_out, granted, free_count_out, pool, tokens, (int)requests, columns,

@@ -119,3 +119,26 @@ def test_step_and_append_arguments():
         args = list(good)
         args[at] = value
         assert lib.tr_append_kv(*args) == status, (at, value)
+
+
+@pytest.mark.parametrize("name", ["tables", "lens", "starts", "lse"])
+def test_attention_index_pointers_off_their_elements(name):
+    a = attention(**{name: P + 2})
+    assert abi.lib().tr_paged_attention(ctypes.byref(a), None, 0, None) == abi.TR_ERR_ALIGN
+
+
+def test_attention_of_more_tokens_than_an_index_holds():
+    # their product with the heads passes 64 bits
+    a = attention(tokens=1 << 62)
+    assert abi.lib().tr_paged_attention(ctypes.byref(a), None, 0, None) == abi.TR_ERR_UNSUPPORTED
+
+
+def test_step_pointers_off_their_elements():
+    lib = abi.lib()
+    good = [P, P, 4, P, 8, 8, P, 100, P, 16, 64, P, P, P, P, P, P, None]
+    for at in (0, 1, 3, 6, 8, 12, 13, 14, 15, 16):
+        assert lib.tr_plan_step(*good[:at], P + 2, *good[at + 1:]) == abi.TR_ERR_ALIGN, at
+    assert lib.tr_plan_step(*good[:11], P + 4, *good[12:]) == abi.TR_ERR_ALIGN
+    good = [P, P, 4, P, 8, 8, P, 100, P, 16, None]
+    for at in (0, 1, 3, 6, 8):
+        assert lib.tr_release_pages(*good[:at], P + 2, *good[at + 1:]) == abi.TR_ERR_ALIGN, at
