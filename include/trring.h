@@ -269,8 +269,10 @@ int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, c
  * first TR_ATTENTION_STATE_BYTES are zeroed once (tr_workspace_clear) and left ready for the
  * next call, of whatever shape; it serves one stream at a time.  Waits inside the kernels are
  * bounded (wait_polls polls, 0 = built-in limit of about a second): one that runs out ends the
- * kernel with TR_ERR_TIMEOUT in the status word (tr_workspace_status); out is then not valid,
- * and the state is zeroed again before the next call.                                        */
+ * kernel with TR_ERR_TIMEOUT in the status word (tr_workspace_status).  What that call did not
+ * finish is NaN in out and lse, and so is all of later calls with the workspace, until its
+ * state is zeroed (tr_workspace_clear of TR_ATTENTION_STATE_BYTES: tr_workspace_status's
+ * `reset`, which clears the word alone, is not enough).                                       */
 #define TR_ATTENTION_STATE_BYTES ((1 << 20) + 256)
 typedef struct tr_attention {
   const void* q;

@@ -17,13 +17,13 @@ paged_attention, residual_norm and sample_tokens, over a paged cache.
 from .spec import (SPEC_C1, SPEC_C2, SPEC_C3, SPEC_C4, SPEC_C5, TRSpec, baseline_cores,
                    baseline_sigma, baseline_x, make_cores, validate, validate_cores)
 from .ring import consume_add, consume_silu_mul, prepare_optimized, tr_forward_optimized
-from .serve import (StepPlan, append_kv, paged_attention, plan_step, release_pages, residual_norm,
-                    sample_tokens)
+from .serve import (StepPlan, append_kv, attention_status, paged_attention, plan_step, release_pages,
+                    residual_norm, sample_tokens, set_attention_wait_limit)
 
 __all__ = [
     "TRSpec", "make_cores", "baseline_cores", "baseline_sigma", "baseline_x", "validate",
     "validate_cores", "prepare_optimized", "tr_forward_optimized", "consume_silu_mul", "consume_add",
     "StepPlan", "plan_step", "release_pages", "append_kv", "paged_attention", "residual_norm",
-    "sample_tokens",
+    "sample_tokens", "attention_status", "set_attention_wait_limit",
     "SPEC_C1", "SPEC_C2", "SPEC_C3", "SPEC_C4", "SPEC_C5",
 ]

@@ -43,8 +43,6 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
-
-
 // Zeros and -inf for the tokens outside [starts[0], starts[requests]); `thread` of `threads`.
 template <typename E>
 __device__ void clear_outside(const tr_attention& a, int64_t thread, int64_t threads) {
@@ -61,6 +59,23 @@ __device__ void clear_outside(const tr_attention& a, int64_t thread, int64_t thr
       const int64_t n = i / a.heads, t = n < first ? n : end + (n - first);
       a.lse[t * a.heads + (i - n * a.heads)] = -INFINITY;
     }
+}
+
+// NaN for `rows` rows from row `row0` of kv head kvh of a request (16-bit types; 0x7fff is NaN in
+// both).  A call that timed out leaves arrival counters behind that are not zero, so neither what it
+// did not finish nor what later calls would join by them may pass for a result: those items are
+// spoiled, by the block whose run they are in, until the workspace's state is zeroed.
+__device__ __forceinline__ void spoil_rows(const tr_attention& a, int64_t token0, int kvh, int g,
+                                           int row0, int rows) {
+  const int per = a.head_dim / 8;
+#pragma unroll 1
+  for (int j = threadIdx.x; j < rows * per; j += blockDim.x) {
+    const int row = row0 + j / per, i = row / g, h = kvh * g + (row - i * g);
+    const int64_t at = (token0 + i) * a.heads + h;
+    reinterpret_cast<uint4*>(a.out)[at * per + j % per] =
+        make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    if (a.lse && j % per == 0) a.lse[at] = __int_as_float(0x7fffffff);
+  }
 }
 
 // The workspace: the status word (tr_workspace_status), the arrival counters of the items, which

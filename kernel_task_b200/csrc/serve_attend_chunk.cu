@@ -30,7 +30,8 @@
 // the last block to arrive, in unit order.
 //
 // Every wait is bounded: when one runs out the block raises its abort flag, all roles leave
-// their loops, tensor memory is freed and the workspace's status word says TR_ERR_TIMEOUT.
+// their loops, tensor memory is freed, the rows of its run become NaN and the workspace's status
+// word says TR_ERR_TIMEOUT; while it does, later calls give NaN too.
 #include <algorithm>
 
 #include "serve_attend.cuh"
@@ -243,7 +244,7 @@ enum {
 template <typename E, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attend_chunk_kernel(const tr_attention a, int* status, int* counters, int64_t max_items,
-                        float* partials, unsigned wait_polls) {
+                        float* partials, unsigned last_poll) {
   constexpr int NS = ring_slots<D>();
   constexpr int QBYTES = kSubRows * D * 2, SLOT = slot_bytes<D>(), CPR = D / 8;
   constexpr int64_t PARTIAL = (int64_t)kTileRows * (D + 2);
@@ -256,6 +257,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.heads / a.kv_heads, R = (int)a.requests;
+  // Whether an earlier call timed out: read by one thread, since a block of this call may set the
+  // word at any time, and on its way while the run is found.  All threads see it after the scans.
+  if (tid == 0) sh_abort = __ldcg(status);
   clear_outside<E>(a, (int64_t)blockIdx.x * kChunkThreads + tid, (int64_t)gridDim.x * kChunkThreads);
   if (R == 0) return;
 
@@ -299,6 +303,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     first_item = it;
   }
 
+  const auto spoil_run = [&] {
+    ChunkItem it = first_item;
+    for (; it.u0 < u_end; next_item(a, g, it))
+      spoil_rows(a, it.token0, it.kvh, g, it.tile * kTileRows,
+                 min(kTileRows, it.rows - it.tile * kTileRows));
+  };
+  if (sh_abort) {
+    __syncthreads();
+    spoil_run();
+    return;
+  }
+
   // ---- set-up
   const auto bar = [&](int i) { return smem_u32(&bars[i]); };
   if (warp == 8) {
@@ -319,7 +335,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     fence_async_smem();
-    if (lane == 0) sh_abort = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -336,7 +351,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     bool ok = true;
     for (unsigned i = 0; ok && !mbar_try_once(bar(b), parity); ++i) {
       if (*abort) ok = false;
-      if (i >= wait_polls) {
+      if (i >= last_poll) {
         *abort = 1;
         ok = false;
       }
@@ -750,7 +765,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512)
                  : "memory");
   }
-  if (tid == 0 && sh_abort) atomicExch(status, (int)TR_ERR_TIMEOUT);
+  if (sh_abort) {
+    if (tid == 0) atomicExch(status, (int)TR_ERR_TIMEOUT);
+    spoil_run();
+  }
 }
 
 // ---- host
@@ -773,7 +791,7 @@ static int launch_chunk(const tr_attention& a, const AttendWorkspace& ws, void* 
   }
   kernel<<<serve_sms(), kChunkThreads, chunk_smem<D>(), static_cast<cudaStream_t>(stream)>>>(
       a, ws.status, ws.counters, attend_chunk_items(a) / 2, ws.partials,
-      a.wait_polls ? a.wait_polls : kChunkWaitPolls);
+      (a.wait_polls ? a.wait_polls : kChunkWaitPolls) - 1);
   return serve_launched("tr_paged_attention");
 }
 

@@ -168,6 +168,7 @@ __device__ __forceinline__ bool find_run(const tr_attention& a, int g, int64_t m
 
 template <typename E, int D, int NT>
 __global__ void __launch_bounds__(kRowsThreads, 2) attend_rows_kernel(const tr_attention a,
+                                                                     const int* status,
                                                                      int* counters,
                                                                      int64_t max_items,
                                                                      float* partials) {
@@ -183,11 +184,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attend_rows_kernel(const tr_a
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = a.heads / a.kv_heads;
+  const int timed_out = __ldcg(status);  // of an earlier call; on its way while the run is found
   clear_outside<E>(a, (int64_t)blockIdx.x * kRowsThreads + tid, (int64_t)gridDim.x * kRowsThreads);
   if (a.requests == 0) return;
   RowsItem it;
   int64_t U, G, u_begin, u_end;
   if (!find_run<ROWS, BK>(a, g, max_items, part, it, U, G, u_begin, u_end)) return;
+  if (timed_out) {
+    for (; it.u0 < u_end; next_item<ROWS, BK>(a, g, it))
+      spoil_rows(a, it.token0, it.kvh, g, it.tile * ROWS, min(ROWS, it.rows - it.tile * ROWS));
+    return;
+  }
 
   const uint32_t stage0 = smem_u32(smem) + warp * STAGES * STAGE;
   float4* exchange = reinterpret_cast<float4*>(smem + kRowsWarps * STAGES * STAGE);
@@ -564,7 +571,7 @@ static int launch_rows(const tr_attention& a, const AttendWorkspace& ws, void* s
     return TR_ERR_CUDA;
   }
   kernel<<<rows_grid(), kRowsThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-      a, ws.counters, rows_max_items(a, 8 * NT), ws.partials);
+      a, ws.status, ws.counters, rows_max_items(a, 8 * NT), ws.partials);
   return serve_launched("tr_paged_attention");
 }
 

@@ -3,6 +3,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdlib>
 #include <map>
@@ -223,19 +224,41 @@ bool checks_status() {
   }();
   return on;
 }
-void check_status(const at::Tensor& ws, const at::Tensor& like, cudaStream_t stream) {
+// The status word of the stream's kept workspace; waits for the stream.  With `reset` a workspace
+// that timed out is given up, and the next call starts from a new one: its counters are not valid
+// any more.
+int64_t attention_status(int64_t device, bool reset) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+  at::Tensor ws;
+  {
+    const std::lock_guard<std::mutex> hold(workspaces_lock);
+    const auto kept = workspaces().find({(int)device, stream});
+    if (kept == workspaces().end()) return TR_OK;
+    ws = kept->second;
+  }
+  int32_t status = TR_OK;
+  check(tr_workspace_status(ws.data_ptr(), ws.numel(), &status, 0, stream), "tr_workspace_status");
+  if (status != TR_OK && reset) {
+    const std::lock_guard<std::mutex> hold(workspaces_lock);
+    const auto kept = workspaces().find({(int)device, stream});
+    if (kept != workspaces().end() && kept->second.is_same(ws)) workspaces().erase(kept);
+  }
+  return status;
+}
+void check_status(const at::Tensor& like, cudaStream_t stream) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess ||
       capture != cudaStreamCaptureStatusNone)
     return;
-  int32_t status = TR_OK;
-  check(tr_workspace_status(ws.data_ptr(), ws.numel(), &status, 0, stream), "tr_workspace_status");
-  if (status == TR_OK) return;
-  const std::lock_guard<std::mutex> hold(workspaces_lock);
-  workspaces().erase({like.get_device(), stream});  // its counters are not valid any more
-  throw std::runtime_error(std::string("paged_attention: ") + tr_status_string(status) +
-                           " (the call's output is not valid)");
+  const int64_t status = attention_status(like.get_device(), true);
+  if (status != TR_OK)
+    throw std::runtime_error(std::string("paged_attention: ") + tr_status_string((int)status) +
+                             " (the call's output is not valid)");
 }
+
+// Polls of a wait before it gives up (0: the built-in limit), for tests of the timeout path.
+std::atomic<uint32_t> attention_polls{0};
 
 std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::Tensor& k_pages,
                                                  const at::Tensor& v_pages,
@@ -289,6 +312,7 @@ std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::
   a.head_dim = (int32_t)D;
   a.dtype = dtype_code(q.scalar_type());
   a.scale = (float)s;
+  a.wait_polls = attention_polls.load(std::memory_order_relaxed);
   size_t bytes = 0;
   check(tr_attention_workspace_bytes(&a, &bytes), "tr_paged_attention");
   cudaStream_t stream = current_stream(q);
@@ -296,7 +320,7 @@ std::pair<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at::
   if (bytes) ws = attention_workspace((int64_t)bytes, q, stream);
   check(tr_paged_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes ? ws.numel() : 0, stream),
         "tr_paged_attention");
-  if (bytes && checks_status()) check_status(ws, q, stream);
+  if (bytes && checks_status()) check_status(q, stream);
   if (!return_lse) return {out, c10::nullopt};
   return {out, lse};
 }
@@ -432,6 +456,9 @@ void bind_serving(py::module_& m) {
   m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
         py::arg("tables"), py::arg("lens"), py::arg("starts"), py::arg("scale") = py::none(),
         py::arg("return_lse") = false);
+  m.def("attention_status", &attention_status, py::arg("device"), py::arg("reset"));
+  m.def("set_attention_wait_limit", [](uint32_t polls) { attention_polls.store(polls); },
+        py::arg("polls"));
   m.def("residual_norm", &residual_norm, py::arg("y"), py::arg("h"), py::arg("post"),
         py::arg("pre"), py::arg("gate"), py::arg("post_bias"), py::arg("pre_bias"),
         py::arg("kind"), py::arg("eps"), py::arg("residual_scale"), py::arg("branch_scale"));

@@ -95,6 +95,26 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return (out, lse) if return_lse else out
 
 
+def attention_status(device: torch.device | str | int | None = None, *, reset: bool = True) -> int:
+    """0, or ``abi.TR_ERR_TIMEOUT`` when a bounded wait inside a ``paged_attention`` on the current
+    stream of ``device`` gave up; waits for the stream.
+
+    What such a call did not finish is NaN, and all that later calls on the stream give, until this
+    function has found the timeout (``reset``: the next call starts from a new workspace).  A call
+    captured in a CUDA graph has a workspace of its own, which every replay zeroes: a timeout shows
+    in the NaN of that replay alone.  With ``TRR_CHECK_STATUS=1`` in the environment every call
+    outside a capture asks by itself, and raises RuntimeError."""
+    d = torch.device("cuda" if device is None else device)
+    return binding().attention_status(torch.cuda.current_device() if d.index is None else d.index,
+                                      reset)
+
+
+def set_attention_wait_limit(polls: int) -> None:
+    """Polls that a wait inside ``paged_attention`` makes before it gives up, in all calls from now on
+    (0: the built-in limit, about a second).  For tests of the timeout path."""
+    binding().set_attention_wait_limit(polls)
+
+
 def residual_norm(y: torch.Tensor | None, h: torch.Tensor, *, post: torch.Tensor | None = None,
                   pre: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                   post_bias: torch.Tensor | None = None, pre_bias: torch.Tensor | None = None,

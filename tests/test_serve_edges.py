@@ -4,6 +4,7 @@ the sizes at which launches change shape, extreme parameters, and state that out
 Tolerances are those of test_serve.py."""
 from __future__ import annotations
 
+import ctypes
 import math
 import os
 import subprocess
@@ -15,8 +16,10 @@ import pytest
 import torch
 
 import kernel_task_b200 as trb
+from kernel_task_b200 import abi
 from test_serve import (attention_case, check_attention, check_plan, check_sample, f64, gen, i32,
                         make_pool, sample_inputs)
+from test_serve_limits import attention_struct, need_of
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
@@ -86,6 +89,96 @@ def test_attention_log_sum_of_a_nan_row_is_nan(new, dim):
     assert out[0, 1].isnan().all() and lse[0, 1].isnan()
     out[0, 1], lse[0, 1] = want[0, 1], want_lse[0, 1]
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def long_chunks():
+    """Prompts and chunks over all SMs, some items shared by blocks; the inputs pass L2 out."""
+    args = attention_case([3000, 2500, 260], [600, 500, 260], 16, 4, 128, 16, torch.bfloat16)
+    torch.cuda.synchronize()
+    torch.empty(64 << 20, device=DEV).fill_(1.0)
+    return args
+
+
+def assert_right_or_nan(out, lse, want, want_lse):
+    """By element: a block that spoils an item it had done its part of may do so while the block
+    that joins the parts writes them, all of them right."""
+    for got, right in ((out, want), (lse, want_lse)):
+        assert (got.isnan() | (got == right)).all()
+    return int(out.isnan().sum())
+
+
+@gpu
+def test_attention_timeout_spoils_what_it_leaves_until_the_state_is_zeroed():
+    args = long_chunks()
+    few = attention_case([3000, 40], [1, 1], 16, 4, 128, 16, torch.bfloat16)
+    want, want_lse = trb.paged_attention(*args, return_lse=True)
+    few_want = trb.paged_attention(*few)
+    out, lse = torch.full_like(want, 7.0), torch.full_like(want_lse, 7.0)
+    few_out = torch.full_like(few_want, 7.0)
+    a, b = attention_struct(args, out, lse, wait_polls=1), attention_struct(few, few_out)
+    need, stream = max(need_of(a), need_of(b)), torch.cuda.current_stream().cuda_stream
+    ws = torch.zeros(need, dtype=torch.uint8, device=DEV)
+
+    def call(s):
+        abi.check(abi.lib().tr_paged_attention(ctypes.byref(s), ctypes.c_void_p(ws.data_ptr()), need,
+                                               ctypes.c_void_p(stream)), "tr_paged_attention")
+
+    def status():
+        return abi.workspace_status(ws.data_ptr(), need, reset=False, stream=stream)
+
+    for polls in (32, 8, 4, 3, 2):  # ends anywhere, or not at all
+        a.wait_polls = polls
+        ws.zero_()
+        call(a)
+        bad = assert_right_or_nan(out, lse, want, want_lse)
+        assert (bad > 0) == (status() == abi.TR_ERR_TIMEOUT)
+    a.wait_polls = 1  # the first loads cannot be there yet
+    ws.zero_()
+    call(a)
+    assert status() == abi.TR_ERR_TIMEOUT
+    assert assert_right_or_nan(out, lse, want, want_lse) > 0
+    a.wait_polls = 0
+    call(a)
+    call(b)
+    assert out.isnan().all() and lse.isnan().all() and few_out.isnan().all()
+    assert status() == abi.TR_ERR_TIMEOUT
+    abi.check(abi.lib().tr_workspace_clear(ctypes.c_void_p(ws.data_ptr()),
+                                           abi.TR_ATTENTION_STATE_BYTES, ctypes.c_void_p(stream)),
+              "tr_workspace_clear")
+    call(a)
+    call(b)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(few_out, few_want)
+    assert status() == abi.TR_OK and not ws[:abi.TR_ATTENTION_STATE_BYTES].any()
+
+
+def binding_timeouts(raises):
+    args = long_chunks()
+    want, want_lse = trb.paged_attention(*args, return_lse=True)
+    assert trb.attention_status() == abi.TR_OK
+    trb.set_attention_wait_limit(1)
+    if raises:
+        with pytest.raises(RuntimeError, match="timed out"):
+            trb.paged_attention(*args)
+    else:
+        got = trb.paged_attention(*args, return_lse=True)
+        assert assert_right_or_nan(*got, want, want_lse) > 0
+    trb.set_attention_wait_limit(0)
+    if not raises:
+        assert trb.paged_attention(*args).isnan().all()
+        assert trb.attention_status(reset=False) == abi.TR_ERR_TIMEOUT
+        with torch.cuda.stream(torch.cuda.Stream()):
+            assert trb.attention_status() == abi.TR_OK
+            assert torch.equal(trb.paged_attention(*args), want)
+            torch.cuda.current_stream().synchronize()
+        assert trb.attention_status() == abi.TR_ERR_TIMEOUT
+    assert trb.attention_status() == abi.TR_OK
+    assert torch.equal(trb.paged_attention(*args), want)
+
+
+@gpu
+@pytest.mark.parametrize("raises", [False, True])
+def test_attention_timeout_through_the_binding(raises):
+    in_fresh_process(f"binding_timeouts({raises})", TRR_CHECK_STATUS=str(int(raises)))
 
 
 # ---------------------------------------------------------------------------------- norms
