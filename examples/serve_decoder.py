@@ -113,9 +113,10 @@ class Decoder:
 
     def step(self, ids: torch.Tensor, new: torch.Tensor, noise: torch.Tensor,
              temperature: torch.Tensor, **limits) -> torch.Tensor:
-        """The next token of every request."""
-        logits, _ = self.forward(ids, new)
-        return sample_tokens(logits, noise, temperature, **limits)[0]
+        """The next token of every request; -1 where it brings none or did not get its pages."""
+        logits, granted = self.forward(ids, new)
+        drawn = sample_tokens(logits, noise, temperature, **limits)[0]
+        return torch.where((granted > 0) & (new > 0), drawn, -1)
 
     def finish(self, done: torch.Tensor) -> None:
         """Give back the pages of the requests with done[r] != 0."""

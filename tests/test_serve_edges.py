@@ -19,6 +19,7 @@ import kernel_task_b200 as trb
 from kernel_task_b200 import abi
 from test_serve import (attention_case, check_attention, check_plan, check_sample, f64, gen, i32,
                         make_pool, sample_inputs)
+from test_serve_decoder import load_example
 from test_serve_limits import attention_struct, need_of
 
 gpu = pytest.mark.gpu
@@ -179,6 +180,20 @@ def binding_timeouts(raises):
 @pytest.mark.parametrize("raises", [False, True])
 def test_attention_timeout_through_the_binding(raises):
     in_fresh_process(f"binding_timeouts({raises})", TRR_CHECK_STATUS=str(int(raises)))
+
+
+# ---------------------------------------------------------------------------- the example
+@gpu
+def test_decoder_draws_no_token_for_idle_and_refused_requests():
+    ex = load_example()
+    model = ex.Decoder(ex.Shape(), 4, pages=8, longest=160)
+    ints = dict(dtype=torch.int32, device=DEV)
+    noise = torch.empty(4, model.shape.vocab, device=DEV).exponential_(generator=gen(3))
+    heat = torch.ones(4, device=DEV)
+    new = [20, 0, 140, 33]  # the third needs nine pages of eight, the fourth comes after it
+    ids = model.step(torch.arange(sum(new), device=DEV), torch.tensor(new, **ints), noise, heat)
+    assert int(ids[0]) >= 0 and ids[1:].tolist() == [-1, -1, -1]
+    assert model.lens.tolist() == [20, 0, 0, 0]
 
 
 # ---------------------------------------------------------------------------------- norms
