@@ -264,7 +264,9 @@ int tr_append_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, c
  * bytes; out [tokens][heads][head_dim] contiguous; tables, pools as above.  Table entries
  * outside [0, pages) read as keys and values of zero; cache rows at and past lens[r] are not
  * used whatever they hold.  head_dim is a multiple of 8 up to 256 (64 and 128 in fp16 and bf16
- * run on tensor cores), page_size a power of two up to 1024, scale positive.
+ * run on tensor cores), page_size a power of two up to 1024, scale positive.  On tensor cores
+ * (tokens g / n + requests) kv_heads is at most 262144, with g = heads / kv_heads and n = 8, or
+ * 16 above 8 rows (tokens g / requests) a request; above 32 rows n is 256 and the limit half.
  * The workspace holds the partial results of contexts that several thread blocks share; its
  * first TR_ATTENTION_STATE_BYTES are zeroed once (tr_workspace_clear) and left ready for the
  * next call, of whatever shape; it serves one stream at a time.  Waits inside the kernels are

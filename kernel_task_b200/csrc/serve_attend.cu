@@ -8,7 +8,11 @@ namespace trr {
 
 // Any head_dim and type: one warp per token and query head, lane l holding elements
 // l, l + 32, ... of q and of the running output, one pass over the keys with the running maximum
-// and sum.  Bound by the five-step reduction of every key's product.
+// and sum.  Bound by the five-step reduction of every key's product, one key after the other: 16
+// requests of 4096, one new token each, 32 heads over 8, take 4.5 ms with a head_dim of 80 or 96
+// in bf16 and of 128 in fp32, 5.6 ms with 256 in bf16 (their bytes: 26 to 83 us; the kernel of
+// serve_attend_rows.cu does 128 in bf16 in 53 us).  It is the form for what the tensor-core kernels
+// do not take, not a fast one.
 template <typename E, int N>
 __global__ void __launch_bounds__(128) attend_generic_kernel(const tr_attention a) {
   const int lane = threadIdx.x & 31;
@@ -80,8 +84,12 @@ static bool on_tensor_cores(const tr_attention& a) {
   return a.dtype != TR_F32 && (a.head_dim == 64 || a.head_dim == 128);
 }
 
-// The chunk kernel from 32 query rows a request and kv head on average, of which its tiles hold
-// 256; the rows kernel below that, where reading the keys is the bound.
+// The chunk kernel above 32 query rows a request and kv head on average, of which its tiles hold
+// 256; the rows kernel up to that, where reading the keys is the bound.  us of the rows kernel /
+// the chunk kernel, 32 heads over 8 of 128 in bf16, with 16, 32 and 64 rows: 8 requests of 8192
+// 54 / 79, 91 / 68, 164 / 71; 32 of 2048 53 / 80, 91 / 68, 140 / 73; one of 8192 25 / 56, 27 / 50,
+// 31 / 50; 4 of 500 14 / 25, 18 / 27, 19 / 29.  The average is the step's: a long prompt takes the
+// requests that decode beside it to the chunk kernel.
 static bool in_chunks(const tr_attention& a) {
   return a.tokens * (a.heads / a.kv_heads) > 32 * a.requests;
 }

@@ -145,12 +145,17 @@ __device__ __forceinline__ void store_row(E* p, int t, int threads, int width,
 
 // A row lies in the registers of its threads (a warp, 8 rows a block; or the block) as N vectors
 // of V elements each, so y and h are read once and both outputs written once whatever the
-// norms need.  A block takes every gridDim.x-th row; where the registers hold it (one vector a
-// thread) it loads the next row before it works on this one, whose sums each cost a barrier,
-// else other blocks of the SM cover them.  The weights come from L1.  Bound by memory: 16384 rows
-// of 4096 from fp32 with a gate per channel take 113 us (6.0 TB/s); 16391 of 2880 with the mean
-// removed and a gate per token 108 us (4.4 TB/s), where the four sums a row are felt (a warp per
-// row of 2880 has no barrier, but 184 us: too few rows in flight); one row 3.8 us.
+// norms need.  A block takes every gridDim.x-th row.  Up to 8 elements a thread (widths to 256, and
+// to 4096 where rows are not vectors) it loads the next row before it works on this one; above, two
+// vectors a thread and more, other blocks of the SM cover the barrier that each sum costs.  The
+// weights come from L1.  Bound by memory: 16384 rows of 4096 from fp32 with a gate per channel
+// take 113 us (6.0 TB/s); 16391 of 2880 with the mean removed and a gate per token 110 us
+// (4.3 TB/s), where the four sums a row are felt (a warp per row of 2880 has no barrier, but
+// 184 us: too few rows in flight); one row 3.8 us.
+// Rows that are not 16-byte vectors are read by elements: 16391 of 2881 from fp16 take 357 us where
+// 2880 take 78 (rms, gate per channel), 8192 of 5001 from fp32 460 us (0.9 TB/s).  Widths above
+// 16384 take 1024 threads of 64 registers and spill (110 to 840 bytes a thread by vectors, 260 to
+// 670 by elements): 1024 rows of 32768 from fp32 83 us (4.0 TB/s), of 32767 405 us.
 template <typename E, typename Y, bool LAYER, bool ROW_WARP, int N, int V, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) residual_norm_kernel(const NormArgs a) {
   constexpr bool AHEAD = N * V <= 8;

@@ -65,9 +65,9 @@ __device__ __forceinline__ Best block_best(Best v, Best* part) {
 }
 
 // For rows that a cluster's shared memory does not hold (over 800000 logits of 16 bits): one block
-// per row, which reads it again for every pass.  Two rows of 900001: about 2 ms.  The cut of top-k and then of top-p is found by radix selection over the
-// ordered keys, 8 bits a pass, counts for the first and masses for the second; ties at the cut
-// are kept in index order.
+// per row, which reads it again for every pass.  Two rows of 900001: about 2 ms.  The cut of
+// top-k and then of top-p is found by radix selection over the ordered keys, 8 bits a pass, counts
+// for the first and masses for the second; ties at the cut are kept in index order.
 template <typename L>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
   __shared__ Best part[32];
@@ -241,7 +241,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 //
 // Every block of the cluster holds a contiguous slice of the logits, so they are read once.  The
 // order of t = logit / temperature is the logits' own, so maxima, histograms and cuts work on
-// the logits; t itself (an exact division) is made for the tokens that reach the final choice.
+// the logits; t itself (an exact division, of the logit less the greatest) is made for the tokens
+// that reach the final choice.  The weights, which every sum of mass is made of (the logprob's
+// normaliser, what top-p cuts by), are one approximate power of two each, off by at most 2^-22 and
+// 2^-23 of the exponent: a cut that two tokens' masses miss by less than that may fall either way.
 //
 // The limits mostly leave few tokens.  Each thread's greatest logit goes into a histogram of 1024
 // steps below the greatest (1/32 of t each), summed over the cluster: these are some of the
@@ -255,11 +258,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 // the kept tokens' probability, and every other draw halves what is left or so.  After
 // kDraws, and for top_k where the mass of what it keeps is asked for, the cut is searched by
 // halving the ordered keys until few enough tokens for a ranked list lie between.
-// All sums run in an order fixed by the row alone.
+// Every sum's order is fixed by the row and by the blocks it is cut over, which the vocabulary and
+// the number of rows decide: the same call gives the same bits, a row sampled alone and in a batch
+// may differ in the last bits of its masses.
 //
-// Bound by instructions and barriers rather than memory: 256 rows of 131072 in bf16 (67 MB, 134 MB
-// of noise) take 44 us greedy, 70 us with top_k 50, 82 us drawn from all tokens (2.5 TB/s); a
-// single row 11 to 17 us, of which five cluster barriers and the launch are most.
+// Bound by instructions and barriers rather than memory: 256 rows of 131072 in bf16 (67 MB, 10.4 us
+// of memory; 134 MB of noise where it is read) take 44 us greedy, 57 us with min_p 0.05, 70 us
+// with top_k 50, 83 us drawn from all tokens (2.4 TB/s), 131 us with top_p 0.9 alone and 209 us
+// with top_k 2000, whose limits need draws and cuts of their own; a single row 10 to 25 us, of
+// which five cluster barriers and the launch are most.
 constexpr int kSliceThreads = 512;
 constexpr int kBins = 1024;
 constexpr float kBinsPerUnit = 32.f;
@@ -607,8 +614,8 @@ __global__ void __launch_bounds__(kSliceThreads, 2) sample_cluster_kernel(const 
 
   if (limited) {
     uint32_t* all = cluster.map_shared_rank(total, 0);
-    // Gathers the tokens from `least` on that `takes(l)` in block 0, if at most kCandidates, and ranks them in its
-    // own_l, own_i; cluster barriers.  Returns their number.
+    // Gathers the tokens from `least` on that `takes(l)` in block 0, if at most kCandidates, and
+    // ranks them in its own_l, own_i; cluster barriers.  Returns their number.
     const auto gather = [&](float least, auto takes) {
       if (tid == 0) sh_count = 0;
       __syncthreads();
@@ -806,7 +813,11 @@ static int launch_sample(const SampleArgs& a, int64_t rows, void* stream) {
     sample_kernel<L><<<(unsigned)rows, kSampleThreads, 0, s>>>(a);
     return serve_launched("tr_sample");
   }
-  // blocks per row: as many as hold it in 64 KB each, more where the rows leave SMs idle
+  // Blocks per row: as many as hold it in 64 KB each, more where the rows leave SMs idle.  Drawn
+  // from all tokens (with top_k 50 and top_p 0.95), us with 2 / 4 / 8 blocks: one row of 50021 in
+  // fp32 14.4 / 12.4 / 10.9 (18.4 / 16.5 / 16.5), 16 rows of 131072 in bf16 24.7 / 16.5 / 15.0
+  // (22.6 / 18.5 / 19.8), 37 rows 26.8 / 21.3 / 26.2 (22.6 / 20.6 / 28.7), 256 rows 122 / 90 / 120
+  // (100 / 79 / 125); 256 rows of 32000 with 1 / 2 / 4 blocks 22 / 29 / 39 (21 / 33 / 51).
   int blocks = 1;
   while (blocks < 8 && (a.vocab * (int)sizeof(L) > blocks * kSliceBytes ||
                         (a.vocab > blocks * 2048 && rows * blocks * 2 <= serve_sms())))

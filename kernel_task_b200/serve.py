@@ -148,8 +148,10 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.
     The token is the kept one with the greatest t - log(noise), which draws it with its
     probability among the kept, or at temperature 0 the one with the greatest logit.  Ranks and
     cuts are those of the logits, also where t no longer tells them apart: an infinite temperature
-    draws evenly among what the limits keep.  Ties of logits go to the lower index everywhere.  The greatest token is always kept; NaN logits count as -inf; a
-    row of nothing but -inf gives token -1.
+    draws evenly among what the limits keep.  Ties of logits go to the lower index everywhere.  The
+    greatest token is always kept; NaN logits count as -inf; a row of nothing but -inf gives token
+    -1.  The same call gives the same bits; a row's masses are summed in an order that depends on
+    the number of rows too, so a cut or a logprob may differ in its last bits between batches.
 
     Returns (tokens int64 [rows], logprobs float32 [rows]): the log of the token's probability
     in the softmax of t over the whole row.
